@@ -22,7 +22,7 @@
 extern "C" {
 #endif
 
-#define SGG_ABI_VERSION 14   /* bump whenever a prototype below changes: tests/abi.lock pins (version, digest of the prototypes) */
+#define SGG_ABI_VERSION 15   /* bump whenever a prototype below changes: tests/abi.lock pins (version, digest of the prototypes) */
 
 enum { SGG_F32 = 0, SGG_BF16 = 1, SGG_F16 = 2,
        /* a PAIR of f16 planes x = hi + lo (hi = f16(x), lo = f16(x - hi): 22 significand bits) -- the operand / activation format of the x3
@@ -402,6 +402,41 @@ int sgg_sgd_multi(float* const* p, const void* const* g, float* const* momentum_
                   const int64_t* n, const float* lr, int count, float weight_decay, float momentum, int first_step,
                   const float* norm_sq, float max_norm, float grad_scale, int g_dtype, int shadow_dtype,
                   int max_blocks /* 0: default 512 */, int* skipped, void* stream);
+
+/* ---- layer normalisation over the last axis (beside the batch / instance normalisations of the GAN's layers) ----
+ * y = (x - mean) / sqrt(var + eps) * w + b per row, var = mean((x - mean)^2); x [M, C] with row stride ldx, y [M, C] contiguous, both `dtype`;
+ * w, b f32[C] or NULL; mean, rstd f32[M] (what the backward reads), both or neither NULL; 1 <= C <= SGG_LAYER_NORM_MAX, eps > 0.
+ * bwd: dx [M, C] contiguous (or NULL), dw, db f32[C] (or NULL), overwritten; dw_j = sum dy xhat, db_j = sum dy, added in a fixed order.
+ * ws: f32[2 * C * sgg_layer_norm_bwd_parts(M, C, dtype)] when dw or db is wanted. */
+#define SGG_LAYER_NORM_MAX 16384
+int sgg_layer_norm_fwd(const void* x, int64_t ldx, const float* w, const float* b, void* y, float* mean, float* rstd, int64_t M, int C, float eps,
+                       int dtype, void* stream);
+int sgg_layer_norm_bwd_parts(int64_t M, int C, int dtype);
+int sgg_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ldx, const float* w, const float* mean, const float* rstd, void* dx,
+                       float* dw, float* db, float* ws, int64_t M, int C, int dtype, void* stream);
+
+/* ---- matrix product in 8-bit floating point (OCP e4m3) with a power-of-two scale for each block of 128 along the reduction ----
+ * Operand form of x [M, K]: `rows` u8 [M][Kp], Kp = K rounded up to 128 (zeros past K), and rows_scale u8 [sgg_fp8_scale_bytes(M, K)]: the
+ * exponent byte e + 127 of each row and block, e >= -126 the smallest with max|x| <= 448 * 2^e over the block's finite elements (non-finite
+ * elements become NaN); byte ((b * G + m / 128) * 32 + m % 32) * 4 + (m / 32) % 4, G = ceil(M / 128).  `cols` / cols_scale: the same form of x^T
+ * ([K][Mp]), out of the same reading of x.  Either form may be NULL (with its scales).  rows, cols 16-byte aligned.
+ * gemm_fp8: C[m][n] = act(sum_k A[m][k] W[n][k] + bias[n]), fp32 accumulation, one rounding to out_dtype; bias f32[N] or NULL; ldc in
+ * elements; ws f32[splits * M * N] when sgg_gemm_fp8_splits(M, N, Kp) is more than 1 (the K slices are added in a fixed order). */
+int64_t sgg_fp8_scale_bytes(int64_t rows, int64_t K);
+int sgg_fp8_quantize(const void* x, int64_t ldx, int64_t M, int64_t K, void* rows, void* rows_scale, void* cols, void* cols_scale, int dtype,
+                     void* stream);
+int sgg_gemm_fp8_splits(int64_t M, int64_t N, int64_t Kp);
+int sgg_gemm_fp8(const void* A, const void* A_scale, const void* W, const void* W_scale, const float* bias, void* C, int64_t ldc, int64_t M, int64_t N,
+                 int64_t Kp, int act, int out_dtype, float* ws, void* stream);
+
+/* ---- global gradient norm over many tensors, and clipping, for an optimiser that is not sgg_sgd_multi ----
+ * norm[0] = |grad_scale| * sqrt(sum of all squares) (squares added in 64 bits, in a fixed order); with `out` (host array of device pointers, entries
+ * may equal g's: in place): out_i = g_i * grad_scale * min(1, max_norm / (norm + 1e-6)).  g, out, n, g_dtype, out_dtype: host arrays of
+ * `count` entries; any alignment of whole elements; no two of the tensors may overlap unless g_i and out_i are the same one of one type.
+ * ws: f64[sgg_clip_grads_parts(count)].  Two launches per 96 tensors. */
+int sgg_clip_grads_parts(int count);
+int sgg_clip_grads(const void* const* g, void* const* out, const int64_t* n, const int* g_dtype, const int* out_dtype, int count, double max_norm,
+                   double grad_scale, double* ws, float* norm, void* stream);
 
 /* x f32 [rows, K] (row stride ldx) -> the PAIR form (SGG_PAIR16): out f16 [rows, 2 * K_pad] = [hi (K_pad) | lo (K_pad)], hi = f16(x),
  * lo = f16(x - hi), columns K .. K_pad - 1 zero.  K_pad % 8 == 0 (the GEMMs want % 64), ldo >= 2 K_pad.  The operand format of the x3 mode

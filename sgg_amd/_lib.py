@@ -5,21 +5,21 @@ product path raises.  The oracle (oracle/) is never imported from here.
 """
 import ctypes
 import os
-from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int, c_int64, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get('SGG_HIP_LIB') or os.path.join(_HERE, 'libsgg_hip.so')   # override: kernel experiments only
 
 SGG_F32, SGG_BF16, SGG_F16 = 0, 1, 2
 ACT_NONE, ACT_RELU = 0, 1
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 import threading  # noqa: E402
 # held by sgg_amd.graph_step while it captures a hipGraph, and by every other thread of this package around its own GPU calls (the
 # DeviceStager's worker: copies, event records): no call of another thread lands in the middle of a stream capture
 CAPTURE_LOCK = threading.RLock()
 
-_P, _I, _F, _L = c_void_p, c_int, c_float, c_int64
+_P, _I, _F, _L, _D = c_void_p, c_int, c_float, c_int64, c_double
 
 # name -> argtypes (all return int unless listed in _RESTYPE)
 SIGNATURES = {
@@ -114,9 +114,18 @@ SIGNATURES = {
     'sgg_sqnorm_acc': [_P, _L, _P, _P, _I, _I, _P],
     'sgg_sgd_step': [_P, _P, _P, _L, _F, _F, _F, _I, _P, _F, _F, _I, _P],
     'sgg_cast': [_P, _P, _L, _I, _I, _P],
+    'sgg_layer_norm_fwd': [_P, _L, _P, _P, _P, _P, _P, _L, _I, _F, _I, _P],
+    'sgg_layer_norm_bwd_parts': [_L, _I, _I],
+    'sgg_layer_norm_bwd': [_P, _L, _P, _L, _P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _P],
+    'sgg_fp8_scale_bytes': [_L, _L],
+    'sgg_fp8_quantize': [_P, _L, _L, _L, _P, _P, _P, _P, _I, _P],
+    'sgg_gemm_fp8_splits': [_L, _L, _L],
+    'sgg_gemm_fp8': [_P, _P, _P, _P, _P, _P, _L, _L, _L, _L, _I, _I, _P, _P],
+    'sgg_clip_grads_parts': [_I],
+    'sgg_clip_grads': [_P, _P, _P, _P, _P, _I, _D, _D, _P, _P, _P],
     'sgg_permute_ncp_to_npc': [_P, _P, _I, _I, _I, _I, _I, _P],
 }
-_RESTYPE = {'sgg_build_info': c_char_p}
+_RESTYPE = {'sgg_build_info': c_char_p, 'sgg_fp8_scale_bytes': c_int64}
 
 _ERRORS = {-1: (ValueError, 'bad argument (size / alignment / null pointer)'),
            -2: (TypeError, 'unsupported element type'),

@@ -27,12 +27,14 @@ from . import ops
 #         split-operand lowering, csrc/util.hip sgg_split3): ~1e-6 relative of exact fp32 -- for operands INSIDE f16's range only (an
 #         unnormalised discriminator whose activations pass 65504 overflows the hi half: measured, tools/dbg_gan.py), and at the GAN's
 #         shapes the split passes cost what the faster products gain (bench.py --mode gqa_gan: 72 ms either way) -- opt-in;
-#   'f16' operands rounded to f16 once, fp32 accumulate (the SGG head's default mode; for the GAN an accuracy trade the caller opts into).
+#   'f16' operands rounded to f16 once, fp32 accumulate (the SGG head's default mode; for the GAN an accuracy trade the caller opts into);
+#   'fp8' operands rounded to 8-bit floating point with a power-of-two scale per 128 values of the reduction, fp32 accumulate, forward and
+#         both gradients (affine_fp8): a relative rounding of 2^-4 per operand value -- for networks trained in it or served from it.
 _COMPUTE = ['f32']
 
 
 def set_compute(mode):
-    assert mode in ('x3', 'f32', 'f16'), mode
+    assert mode in ('x3', 'f32', 'f16', 'fp8'), mode
     prev = _COMPUTE[0]
     _COMPUTE[0] = mode
     return prev
@@ -45,6 +47,8 @@ def compute_mode():
 def product(x, w, bias=None):
     """x [M,Kp] f32 . w [N,Kp]^T (+ bias) -> [M,N] f32 in the file's arithmetic (Kp a multiple of 32, zero-padded)"""
     mode = _COMPUTE[0]
+    if mode == 'fp8':
+        return ops.gemm_fp8(ops.quantize_fp8(x), ops.quantize_fp8(w), bias)
     if mode == 'f16':
         x16, w16 = ops.cast(x, torch.float16), ops.cast(w, torch.float16)
         if x16.shape[1] % 64:
@@ -116,10 +120,75 @@ class _Affine(torch.autograd.Function):
         return dx, dw, db
 
 
+def _row_form(x):
+    """a row matrix the kernels can address (contiguous rows that do not overlap), copied only where it is not one"""
+    x = x.detach()
+    M, K = x.shape
+    return x if (K <= 1 or x.stride(1) == 1) and (M <= 1 or x.stride(0) >= K) else x.contiguous()
+
+
+class _AffineFp8(torch.autograd.Function):
+    """y = Q(x) . Q(w)^T + b, dx = Q(dy) . Q(w^T)^T, dw = Q(dy^T) . Q(x^T)^T, db = column sums of dy, Q the 8-bit operand form (ops.quantize_fp8:
+    blocks of 128 along each product's own reduction, so x, w and dy are read once and written in both orders).  What the backward
+    keeps of x and w is their 8-bit transposes."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, out_dtype):
+        _need_gpu(x)
+        if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+            raise ValueError('dense: inputs %s against weights %s' % (tuple(x.shape), tuple(w.shape)))
+        xr, wr = _row_form(x), _row_form(w)
+        need_dx, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        xq, xt = ops.quantize_fp8(xr, 'both') if need_dw else (ops.quantize_fp8(xr), None)
+        wq, wt = ops.quantize_fp8(wr, 'both') if need_dx else (ops.quantize_fp8(wr), None)
+        ctx.save_for_backward(*[t for q in (xt, wt) if q is not None for t in (q.data, q.scale)])
+        ctx.kept = tuple(None if q is None else q.shape for q in (xt, wt))
+        ctx.types = (x.dtype, w.dtype, b.dtype if b is not None else None)
+        return ops.gemm_fp8(xq, wq, b.detach().float().contiguous() if b is not None else None, out_dtype=out_dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        saved = iter(ctx.saved_tensors)
+        xt, wt = [None if shape is None else ops.Fp8Rows(next(saved), next(saved), shape) for shape in ctx.kept]
+        need_dx, need_dw, need_db = ctx.needs_input_grad[:3]
+        need_dx, need_dw = need_dx and wt is not None, need_dw and xt is not None
+        dy = _row_form(dy)
+        dq = dt = dx = dw = db = None
+        if need_dx and need_dw:
+            dq, dt = ops.quantize_fp8(dy, 'both')
+        elif need_dx:
+            dq = ops.quantize_fp8(dy)
+        elif need_dw:
+            dt = ops.quantize_fp8(dy, 'cols')
+        if need_dx:
+            dx = ops.gemm_fp8(dq, wt, out_dtype=ctx.types[0])
+        if need_dw:
+            dw = ops.gemm_fp8(dt, xt).to(ctx.types[1])
+        if need_db:
+            db = (ops.colsum(dy.contiguous()) if dy.shape[0] else dy.new_zeros(dy.shape[1], dtype=torch.float32)).to(ctx.types[2])
+        return dx, dw, db, None
+
+
+def affine_fp8(x, weight, bias=None, out_dtype=None):
+    """x [..., K] (f32 / bf16 / f16) -> [..., N] = x . weight^T + bias in 8-bit floating point (ops.gemm_fp8), out_dtype (default x's type);
+    differentiable in all three, the gradients' products in 8 bits too.  What set_compute('fp8') makes of affine / conv2d."""
+    _need_gpu(x)
+    y = _AffineFp8.apply(x.reshape(-1, x.shape[-1]), weight, bias, out_dtype or x.dtype)
+    return y.view(*x.shape[:-1], weight.shape[0])
+
+
+def _affine_rows(x, w, b):
+    """the product of a row matrix in the file's arithmetic (columns of x past w's are zero: a padded patch matrix)"""
+    if _COMPUTE[0] != 'fp8':
+        return _Affine.apply(x, w, b)
+    return _AffineFp8.apply(x, w if w.shape[1] == x.shape[1] else F.pad(w, (0, x.shape[1] - w.shape[1])), b, torch.float32)
+
+
 def affine(x, weight, bias=None):
-    """x [..., K] -> [..., N] = x . weight^T + bias (weight [N,K]) on sgg_gemm; differentiable in all three."""
+    """x [..., K] -> [..., N] = x . weight^T + bias (weight [N,K]) on sgg_gemm (sgg_gemm_fp8 in the 'fp8' arithmetic); differentiable in all three."""
     lead = x.shape[:-1]
-    y = _Affine.apply(x.reshape(-1, x.shape[-1]), weight, bias)
+    y = _affine_rows(x.reshape(-1, x.shape[-1]), weight, bias)
     return y.view(*lead, weight.shape[0])
 
 
@@ -153,7 +222,7 @@ def conv2d(x, weight, bias=None, padding=0, stride=1):
         wmat = weight.permute(0, 2, 3, 1).reshape(Cout, k * k * C)       # columns in the patch matrix's (ky, kx, c) order
         if rows.shape[1] != wmat.shape[1]:
             wmat = F.pad(wmat, (0, rows.shape[1] - wmat.shape[1]))
-    return _Affine.apply(rows, wmat, bias).view(B, Ho, Wo, Cout)
+    return _affine_rows(rows, wmat, bias).view(B, Ho, Wo, Cout)
 
 
 # ------------------------------------------------------------------------------------------------ modules
@@ -241,6 +310,43 @@ class BatchNormRows(nn.modules.batchnorm._BatchNorm):
         if self.affine:
             y = y + self.bias
         return y.view(x.shape)
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, b, eps):
+        xr = _row_form(x)
+        need = any(ctx.needs_input_grad[:3])
+        y, mean, rstd = ops.layer_norm(xr, w, b, eps, stats=need)
+        if need:
+            ctx.save_for_backward(xr, mean, rstd, *([w] if w is not None else []))
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        xr, mean, rstd = ctx.saved_tensors[:3]
+        w = ctx.saved_tensors[3] if len(ctx.saved_tensors) > 3 else None
+        return ops.layer_norm_bwd(_row_form(dy), xr, mean, rstd, w, *ctx.needs_input_grad[:3]) + (None,)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """Layer normalisation over the last axis of x [..., C] (f32 / bf16 / f16; statistics and sums in fp32) with weight, bias f32[C] or None
+    -> x's shape and type; differentiable in all three (csrc/layernorm.hip: one pass each way)."""
+    _need_gpu(x)
+    return _LayerNorm.apply(x.reshape(-1, x.shape[-1]), weight, bias, eps).view(x.shape)
+
+
+class LayerNormRows(nn.LayerNorm):
+    """nn.LayerNorm over the last axis (its parameters and state names) on layer_norm: row matrices [M,C] and channels-last maps alike"""
+
+    def __init__(self, num_features, eps=1e-5, elementwise_affine=True):
+        super(LayerNormRows, self).__init__(num_features, eps=eps, elementwise_affine=elementwise_affine)
+
+    def forward(self, x):
+        if x.shape[-1] != self.normalized_shape[0]:
+            raise ValueError('LayerNormRows(%d) got %d columns' % (self.normalized_shape[0], x.shape[-1]))
+        return layer_norm(x, self.weight, self.bias, self.eps)
 
 
 class RowsSyncBatchNorm(nn.SyncBatchNorm):

@@ -414,7 +414,7 @@ def gan_train_step(sgg_model, gan, res, gt_boxes, gt_objects, gt_rels, optimizer
     BatchNorm1d of the graph convolutions when BN=True) use batch statistics: convert them with
     `sgg_amd.dense.sync_batchnorm_(gan)` (the channels-last counterpart of torch.nn.SyncBatchNorm.convert_sync_batchnorm) for
     statistics over every rank's images (what the test does), or keep replica-local statistics."""
-    from .trainer import Trainer
+    from .trainer import Trainer, clip_grad_norm_
     import torch.distributed as dist
     world = _dp_world()
     gan.train()
@@ -481,7 +481,7 @@ def gan_train_step(sgg_model, gan, res, gt_boxes, gt_objects, gt_rels, optimizer
                 else:
                     allreduce_grads_([p for p in sgg_model.parameters() if p.requires_grad])
                     if clip:
-                        torch.nn.utils.clip_grad_norm_([p for p in sgg_model.parameters() if p.grad is not None], clip)
+                        clip_grad_norm_(sgg_model.parameters(), clip)
                     optimizer.step()
             allreduce_grads_(G_params, 1.0 / scale)
             # a scaled f16 backward that overflowed: the SGG update above was skipped by its norm check; the generator's optimiser has no

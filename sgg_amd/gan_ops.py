@@ -115,8 +115,9 @@ def triple_pool(new_t_vecs, edges, num_objs, hidden_dim, o_off, pooling='avg'):
 
 
 def build_mlp(dim_list, activation='relu', batch_norm='none', dropout=0, final_nonlinearity=True):
-    """graphconv.py:157-176: Linear [BatchNorm1d] [ReLU | LeakyReLU] ... with the reference's Sequential indices (checkpoints load).
-    The Linear layers multiply on this package's GEMM (sgg_amd/dense.py), the normalisation is its row-matrix BatchNorm."""
+    """graphconv.py:157-176: Linear [BatchNorm1d | layer norm] [ReLU | LeakyReLU] ... with the reference's Sequential indices (checkpoints load).
+    The Linear layers multiply on this package's GEMM (sgg_amd/dense.py), the normalisation is its row-matrix BatchNorm
+    ('batch') or, beside the reference's choices, its layer norm ('layer')."""
     from . import dense
     act = {'relu': torch.nn.ReLU, 'leakyrelu': torch.nn.LeakyReLU}.get(activation)
     layers = []
@@ -126,6 +127,8 @@ def build_mlp(dim_list, activation='relu', batch_norm='none', dropout=0, final_n
         if i < n_layers - 1 or final_nonlinearity:
             if batch_norm == 'batch':
                 layers.append(dense.BatchNormRows(d_out))
+            elif batch_norm == 'layer':                      # statistics of one row: no batch, nothing to synchronise over ranks
+                layers.append(dense.LayerNormRows(d_out))
             if act is not None:
                 layers.append(act())
         if dropout > 0:

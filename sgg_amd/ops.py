@@ -1165,3 +1165,216 @@ def add_relu_(y, x):
     assert y.shape == x.shape and y.dtype == x.dtype
     _lib.call('sgg_add_relu', _p(y), _p(x), y.numel(), dt(y), _stream())
     return y
+
+
+# ---------------------------------------------------------------- low-precision dense training: layer norm, 8-bit products, clipping
+LAYER_NORM_MAX = 16384      # include/sgg_hip.h SGG_LAYER_NORM_MAX: widest row of layer_norm
+FP8_BLOCK = 128             # columns that share a scale
+
+
+def _here(t, what):
+    """the launch goes to the current device's stream: a tensor of another device is refused, not run there"""
+    if not t.is_cuda:
+        raise RuntimeError('sgg_amd: %s: tensor is not on the GPU (the HIP path has no CPU fallback)' % what)
+    if t.device.index != torch.cuda.current_device():
+        raise RuntimeError('sgg_amd: %s: tensor is on %s, the current device is cuda:%d' % (what, t.device, torch.cuda.current_device()))
+
+
+def _row_matrix(t, what):
+    """row stride of a 2-D tensor whose rows are contiguous and do not overlap"""
+    if t.dim() != 2:
+        raise ValueError('sgg_amd: %s: expected a matrix, got shape %s' % (what, tuple(t.shape)))
+    M, C = t.shape
+    if t.numel() == 0:                           # (an empty tensor's strides say nothing)
+        return C
+    if (C > 1 and t.stride(1) != 1) or (M > 1 and t.stride(0) < C):
+        raise ValueError('sgg_amd: %s: rows must be contiguous and must not overlap (strides %s)' % (what, tuple(t.stride())))
+    return t.stride(0) if M > 1 else C
+
+
+def _vector(t, n, what):
+    if t is None:
+        return None
+    _here(t, what)
+    if tuple(t.shape) != (n,):
+        raise ValueError('sgg_amd: %s: expected shape (%d,), got %s' % (what, n, tuple(t.shape)))
+    return _p(t, torch.float32)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, stats=True):
+    """x [M, C] (f32 / bf16 / f16, row-strided ok) -> (y [M, C] in x's type, mean f32[M], rstd f32[M]); weight, bias f32[C] or None.
+    stats=False: (y, None, None)."""
+    _here(x, 'layer_norm')
+    ld, (M, C) = _row_matrix(x, 'layer_norm'), x.shape
+    if not 1 <= C <= LAYER_NORM_MAX:
+        raise ValueError('sgg_amd: layer_norm: rows of 1 .. %d columns, got %d' % (LAYER_NORM_MAX, C))
+    w, b = _vector(weight, C, 'layer_norm weight'), _vector(bias, C, 'layer_norm bias')
+    y = torch.empty((M, C), dtype=x.dtype, device=x.device)
+    mean, rstd = torch.empty((2, M), dtype=torch.float32, device=x.device) if stats else (None, None)
+    _lib.call('sgg_layer_norm_fwd', x.data_ptr(), ld, w, b, y.data_ptr(), mean.data_ptr() if stats else None, rstd.data_ptr() if stats else None,
+              M, C, float(eps), dt(x), _stream())
+    return y, mean, rstd
+
+
+def layer_norm_bwd(dy, x, mean, rstd, weight=None, want_dx=True, want_dw=True, want_db=True):
+    """the adjoint of layer_norm: dy, x [M, C] of one type, mean / rstd f32[M] as it returned them -> (dx [M, C], dw f32[C], db f32[C]),
+    None for what is not wanted.  The sums over the rows are added in a fixed order: same inputs, same bits."""
+    _here(x, 'layer_norm_bwd')
+    _here(dy, 'layer_norm_bwd')
+    ld, ld_dy, (M, C) = _row_matrix(x, 'layer_norm_bwd'), _row_matrix(dy, 'layer_norm_bwd'), x.shape
+    if tuple(dy.shape) != (M, C) or dy.dtype != x.dtype:
+        raise ValueError('sgg_amd: layer_norm_bwd: dy %s %s against x %s %s' % (tuple(dy.shape), dy.dtype, (M, C), x.dtype))
+    if not 1 <= C <= LAYER_NORM_MAX:
+        raise ValueError('sgg_amd: layer_norm_bwd: rows of 1 .. %d columns, got %d' % (LAYER_NORM_MAX, C))
+    mu, r, w = _vector(mean, M, 'layer_norm_bwd mean'), _vector(rstd, M, 'layer_norm_bwd rstd'), _vector(weight, C, 'layer_norm_bwd weight')
+    dx = torch.empty((M, C), dtype=x.dtype, device=x.device) if want_dx else None
+    dw = torch.empty(C, dtype=torch.float32, device=x.device) if want_dw else None
+    db = torch.empty(C, dtype=torch.float32, device=x.device) if want_db else None
+    ws = None
+    if want_dw or want_db:
+        parts = _lib.load().sgg_layer_norm_bwd_parts(M, C, dt(x))
+        _lib.check(min(parts, 0), 'sgg_layer_norm_bwd_parts')
+        ws = _ws(2 * C * parts, x.device)
+    if want_dx or ws is not None:
+        _lib.call('sgg_layer_norm_bwd', dy.data_ptr(), ld_dy, x.data_ptr(), ld, w, mu, r, _p(dx), _p(dw), _p(db), _p(ws), M, C, dt(x), _stream())
+    return dx, dw, db
+
+
+class Fp8Rows(object):
+    """A matrix [M, K] in the 8-bit operand form of include/sgg_hip.h: `data` float8_e4m3fn [M, K rounded up to 128], `scale` the exponent
+    bytes of its blocks of 128 columns (the kernels' order), `shape` = (M, K)."""
+    __slots__ = ('data', 'scale', 'shape')
+
+    def __init__(self, data, scale, shape):
+        self.data, self.scale, self.shape = data, scale, tuple(shape)
+
+    def exponents(self):
+        """-> int32 [M, blocks]: block b of row m stands for its e4m3 values times 2^exponents[m, b]"""
+        M, blocks = self.shape[0], self.data.shape[1] // FP8_BLOCK
+        e = self.scale.view(blocks, -1, 32, 4).permute(1, 3, 2, 0).reshape(-1, blocks)        # (block, group, r % 32, r / 32) -> rows
+        return e[:M].int() - 127
+
+    def dequantize(self):
+        """-> f64 [M, K], the values the operand stands for, each of them exact (fp32's largest rounds to 2^128, which fp32 has not)"""
+        M, K = self.shape
+        e = ((self.exponents().long() + 1023) << 52).view(torch.float64)                      # 2^e itself
+        return (self.data.float().double().view(M, -1, FP8_BLOCK) * e[:, :, None]).reshape(M, self.data.shape[1])[:, :K]
+
+
+def _fp8_empty(M, K, device):
+    Kp = (K + FP8_BLOCK - 1) // FP8_BLOCK * FP8_BLOCK
+    return Fp8Rows(torch.empty((M, Kp), dtype=torch.float8_e4m3fn, device=device),
+                   torch.empty(_lib.load().sgg_fp8_scale_bytes(M, K), dtype=torch.uint8, device=device), (M, K))
+
+
+def quantize_fp8(x, form='rows'):
+    """x [M, K] (f32 / bf16 / f16, row-strided ok) -> its 8-bit operand form: form 'rows' Fp8Rows of x, 'cols' Fp8Rows of x^T (blocks of 128
+    rows of x share a scale), 'both' the pair of them out of one reading of x.  Non-finite elements become NaN."""
+    if form not in ('rows', 'cols', 'both'):
+        raise ValueError("sgg_amd: quantize_fp8: form must be 'rows', 'cols' or 'both', got %r" % (form,))
+    _here(x, 'quantize_fp8')
+    ld, (M, K) = _row_matrix(x, 'quantize_fp8'), x.shape
+    code = dt(x)
+    r = _fp8_empty(M, K, x.device) if form != 'cols' else None
+    c = _fp8_empty(K, M, x.device) if form != 'rows' else None
+    if M and K:
+        _lib.call('sgg_fp8_quantize', x.data_ptr(), ld, M, K, r.data.data_ptr() if r else None, r.scale.data_ptr() if r else None,
+                  c.data.data_ptr() if c else None, c.scale.data_ptr() if c else None, code, _stream())
+    return r if c is None else c if r is None else (r, c)
+
+
+def gemm_fp8(A, W, bias=None, act=ACT_NONE, out_dtype=torch.float32, out=None):
+    """act(A . W^T + bias) of two Fp8Rows A [M, K], W [N, K] -> [M, N] in out_dtype (or into `out`, row-strided ok): fp32 accumulation, one
+    rounding at the end; bias f32[N]."""
+    if not isinstance(A, Fp8Rows) or not isinstance(W, Fp8Rows):
+        raise TypeError('sgg_amd: gemm_fp8: operands are Fp8Rows (quantize_fp8), got %s and %s' % (type(A).__name__, type(W).__name__))
+    (M, K), N = A.shape, W.shape[0]
+    if W.shape[1] != K:
+        raise ValueError('sgg_amd: gemm_fp8: %s . %s^T' % (A.shape, W.shape))
+    for t in (A.data, A.scale, W.data, W.scale):
+        _here(t, 'gemm_fp8')
+    b = _vector(bias, N, 'gemm_fp8 bias')
+    if out is None:
+        out = torch.empty((M, N), dtype=out_dtype, device=A.data.device)
+    else:
+        _here(out, 'gemm_fp8 out')
+        if tuple(out.shape) != (M, N):
+            raise ValueError('sgg_amd: gemm_fp8: out %s for a [%d, %d] product' % (tuple(out.shape), M, N))
+    ldc, code = _row_matrix(out, 'gemm_fp8 out'), dt(out)
+    Kp = A.data.shape[1]
+    splits = _lib.load().sgg_gemm_fp8_splits(M, N, Kp)
+    _lib.check(min(splits, 0), 'sgg_gemm_fp8_splits')
+    ws = _ws(splits * M * N, out.device) if splits > 1 else None
+    _lib.call('sgg_gemm_fp8', _p(A.data), _p(A.scale), _p(W.data), _p(W.scale), b, out.data_ptr(), ldc, M, N, Kp, act, code, _p(ws), _stream())
+    return out
+
+
+def _dense_layout(t):
+    """elements fill one memory range (whatever the order of the axes)"""
+    return t.is_contiguous() or (t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last))
+
+
+def _grad_list(grads, what):
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    dev = torch.cuda.current_device() if grads else None
+    for g in grads:
+        if not g.is_cuda or g.device.index != dev:
+            _here(g, what)
+        if g.layout != torch.strided:
+            raise TypeError('sgg_amd: %s: dense gradients only (got %s)' % (what, g.layout))
+    return grads
+
+
+def _clip_call(grads, outs, max_norm, grad_scale):
+    import numpy as np
+    n = len(grads)
+    norm = torch.empty((), dtype=torch.float32, device='cuda')
+    ws = torch.empty(_lib.load().sgg_clip_grads_parts(n), dtype=torch.float64, device='cuda')
+    gp = np.array([g.data_ptr() for g in grads], dtype=np.uint64)
+    nn = np.array([g.numel() for g in grads], dtype=np.int64)
+    gd = np.array([dt(g) for g in grads], dtype=np.int32)
+    op = od = None
+    if outs is not None:
+        op, od = (gp, gd) if outs is grads else (np.array([o.data_ptr() for o in outs], dtype=np.uint64), np.array([dt(o) for o in outs], dtype=np.int32))
+        # every tensor is written by workgroups of its own: no two of them may share memory (one given twice would be scaled twice)
+        lo, hi = gp, gp + nn.astype(np.uint64) * np.where(gd == SGG_F32, 4, 2).astype(np.uint64)
+        if op is not gp:
+            apart = (op != gp) | (od != gd)
+            lo = np.concatenate((lo, op[apart]))
+            hi = np.concatenate((hi, (op + nn.astype(np.uint64) * np.where(od == SGG_F32, 4, 2).astype(np.uint64))[apart]))
+        order = np.argsort(lo[hi > lo], kind='stable')
+        a, b = lo[hi > lo][order], hi[hi > lo][order]
+        if (a[1:] < b[:-1]).any():
+            raise ValueError('sgg_amd: clip_grads_: two of the tensors share memory')
+    _lib.call('sgg_clip_grads', gp.ctypes.data, op.ctypes.data if op is not None else None, nn.ctypes.data, gd.ctypes.data,
+              od.ctypes.data if od is not None else None, n, float(max_norm), float(grad_scale), ws.data_ptr(), norm.data_ptr(), _stream())
+    return norm
+
+
+def grad_norm(grads, grad_scale=1.0):
+    """|grad_scale| * the L2 norm over every element of the tensors (f32 / bf16 / f16, mixed) -> f32 scalar on the device, no host
+    synchronisation.  Squares are added in 64 bits and in a fixed order."""
+    grads = [g if _dense_layout(g) else g.contiguous() for g in _grad_list(grads, 'grad_norm')]
+    return _clip_call(grads, None, 0.0, grad_scale)
+
+
+def clip_grads_(grads, max_norm, grad_scale=1.0, out=None):
+    """Global-norm clipping: every gradient times grad_scale * min(1, max_norm / (norm + 1e-6)), norm = grad_norm(grads, grad_scale), in place or
+    into `out` (tensors of the gradients' shapes and memory order, any of the three types: the f16 gradients of a scaled loss become
+    unscaled fp32 ones).  -> norm, f32 scalar on the device.  Nothing waits for the GPU.  A non-finite norm is not hidden: a NaN norm
+    makes every gradient NaN, an infinite one makes them 0 (and NaN where they were infinite), as torch.nn.utils.clip_grad_norm_ does."""
+    grads = _grad_list(grads, 'clip_grads_')
+    if not max_norm >= 0:
+        raise ValueError('sgg_amd: clip_grads_: max_norm must be >= 0, got %r' % (max_norm,))
+    outs = grads if out is None else _grad_list(out, 'clip_grads_ out')
+    if len(outs) != len(grads):
+        raise ValueError('sgg_amd: clip_grads_: %d gradients, %d outputs' % (len(grads), len(outs)))
+    for g, o in zip(grads, outs):
+        if not _dense_layout(g):
+            raise ValueError('sgg_amd: clip_grads_: gradient of shape %s has gaps or overlaps (strides %s)' % (tuple(g.shape), tuple(g.stride())))
+        if o is not g and (o.shape != g.shape or o.stride() != g.stride()):
+            raise ValueError('sgg_amd: clip_grads_: out %s %s for a gradient %s %s' % (tuple(o.shape), tuple(o.stride()), tuple(g.shape), tuple(g.stride())))
+    norm = _clip_call(grads, outs, max_norm, grad_scale)
+    if outs:
+        torch.autograd.graph.increment_version(outs)          # written through raw pointers
+    return norm

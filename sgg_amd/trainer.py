@@ -16,6 +16,14 @@ from . import _lib, ops
 from .dist import GradBuckets, sum_over_ranks
 
 
+def clip_grad_norm_(parameters, max_norm, grad_scale=1.0):
+    """torch.nn.utils.clip_grad_norm_ (L2, lib/pytorch_misc.py:625-656) for an optimiser other than FusedSGD, on ops.clip_grads_: the gradients of
+    `parameters` (a tensor or an iterable; None gradients are passed over) times grad_scale * min(1, max_norm / (norm + 1e-6)), in place; -> norm of
+    the gradients times grad_scale, f32 scalar on the device.  grad_scale: 1 / loss scale of a scaled backward."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
+    return ops.clip_grads_([p.grad for p in parameters if p.grad is not None], max_norm, grad_scale)
+
+
 class FusedSGD(torch.optim.Optimizer):
     """torch.optim.SGD(momentum, weight_decay) + clip_grad_norm (lib/pytorch_misc.py:625-656) as HIP kernels.
 
