@@ -7,7 +7,8 @@ namespace {
 
 constexpr int CLIP_TAB = 96;            // tensors per launch (the table travels by value in the kernel arguments)
 constexpr int CLIP_CHUNK = 8192;        // elements a workgroup takes at a time
-constexpr int CLIP_BLOCKS = 1024;       // partials per launch
+constexpr int CLIP_BLOCKS = 1024;       // partials per launch: 4 workgroups per CU
+constexpr int CLIP_SMALL = 8;           // chunks up to which one workgroup does it all
 
 struct ClipTab {
     const void* g[CLIP_TAB];
@@ -28,6 +29,9 @@ __device__ __forceinline__ int clip_find(const ClipTab& t, int c) {      // the 
     return lo;
 }
 
+typedef u32x4 u32x4_any __attribute__((aligned(2)));       // 16 bytes at the alignment of an element: this chip's loads and stores need no more
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+
 __device__ __forceinline__ float clip_ld(const void* p, long i, int dt) {
     return dt == SGG_F32 ? ((const float*)p)[i] : dt == SGG_BF16 ? bf16_to_f32(((const bf16_t*)p)[i]) : (float)((const f16_t*)p)[i];
 }
@@ -36,57 +40,134 @@ __device__ __forceinline__ void clip_st(void* p, long i, int dt, float v) {
     else if (dt == SGG_BF16) ((bf16_t*)p)[i] = f32_to_bf16(v);
     else ((f16_t*)p)[i] = (f16_t)v;
 }
+__device__ __forceinline__ void clip_st8(void* p, long i, int dt, const float (&v)[8]) {
+    if (dt == SGG_F32) {
+        __builtin_nontemporal_store(f32x4{v[0], v[1], v[2], v[3]}, reinterpret_cast<f32x4_any*>((float*)p + i));
+        __builtin_nontemporal_store(f32x4{v[4], v[5], v[6], v[7]}, reinterpret_cast<f32x4_any*>((float*)p + i + 4));
+    } else {
+        __builtin_nontemporal_store(dt == SGG_BF16 ? pack8<bf16_t>(v) : pack8<f16_t>(v), reinterpret_cast<u32x4_any*>((unsigned short*)p + i));
+    }
+}
 
-__device__ __forceinline__ double clip_block_sum(double v, double* red) {       // 256 threads; every thread gets the sum
+// Walks chunk c of tensor t with THREADS threads: f8(values, index) for whole pieces of 8, f1(value, index) for the elements of a last, partial
+// one.  All of a thread's loads are issued before its first value is used.
+template <int THREADS, typename F8, typename F1>
+__device__ __forceinline__ void clip_walk(const ClipTab& tab, int t, int c, F8&& f8, F1&& f1) {
+    const long base = (long)(c - tab.chunk0[t]) * CLIP_CHUNK;
+    const int left = (int)min((long)CLIP_CHUNK, tab.n[t] - base), dt = tab.gdt[t];
+    constexpr int PASS = CLIP_CHUNK / (THREADS * 8);
+    const char* p = (const char*)tab.g[t] + base * (dt == SGG_F32 ? 4 : 2);
+    const int at = threadIdx.x * 8;
+    if (dt == SGG_F32) {
+        f32x4 r[PASS][2];
+#pragma unroll
+        for (int q = 0; q < PASS; ++q)
+            if (q * THREADS * 8 + at + 8 <= left) {
+                const float* e = (const float*)p + q * THREADS * 8 + at;
+                r[q][0] = *reinterpret_cast<const f32x4_any*>(e);
+                r[q][1] = *reinterpret_cast<const f32x4_any*>(e + 4);
+            }
+#pragma unroll
+        for (int q = 0; q < PASS; ++q)
+            if (q * THREADS * 8 + at + 8 <= left) {
+                const float v[8] = {r[q][0].x, r[q][0].y, r[q][0].z, r[q][0].w, r[q][1].x, r[q][1].y, r[q][1].z, r[q][1].w};
+                f8(v, base + q * THREADS * 8 + at);
+            }
+    } else {
+        u32x4 r[PASS];
+#pragma unroll
+        for (int q = 0; q < PASS; ++q)
+            if (q * THREADS * 8 + at + 8 <= left) r[q] = *reinterpret_cast<const u32x4_any*>((const unsigned short*)p + q * THREADS * 8 + at);
+#pragma unroll
+        for (int q = 0; q < PASS; ++q)
+            if (q * THREADS * 8 + at + 8 <= left) {
+                float v[8];
+                if (dt == SGG_BF16) unpack8<bf16_t>(r[q], v);
+                else unpack8<f16_t>(r[q], v);
+                f8(v, base + q * THREADS * 8 + at);
+            }
+    }
+    if ((int)threadIdx.x < (left & 7)) f1(clip_ld(p, (left & ~7) + threadIdx.x, dt), base + (left & ~7) + threadIdx.x);
+}
+
+template <int THREADS>
+__device__ __forceinline__ double clip_block_sum(double v, double* red) {       // every thread gets the sum
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
-    return (red[0] + red[1]) + (red[2] + red[3]);
+    v = red[0];
+#pragma unroll
+    for (int i = 1; i < THREADS / 64; ++i) v += red[i];
+    return v;
 }
 
-__global__ __launch_bounds__(256) void clip_norm_kernel(const ClipTab tab, double* __restrict__ part) {
-    __shared__ double red[4];
+template <int THREADS>
+__device__ __forceinline__ double clip_squares(const ClipTab& tab, int first, int step) {
     const int total = tab.chunk0[tab.count];
-    double s = 0.0;
-    for (int c = blockIdx.x; c < total; c += gridDim.x) {
-        const int t = clip_find(tab, c);
-        const long base = (long)(c - tab.chunk0[t]) * CLIP_CHUNK, end = min(tab.n[t], base + CLIP_CHUNK);
-        for (long i = base + threadIdx.x; i < end; i += 256) {
-            const double v = (double)clip_ld(tab.g[t], i, tab.gdt[t]);
-            s = fma(v, v, s);
-        }
-    }
-    s = clip_block_sum(s, red);
-    if (threadIdx.x == 0) part[blockIdx.x] = s;
+    double s[2] = {0.0, 0.0};
+    for (int c = first; c < total; c += step)
+        clip_walk<THREADS>(tab, clip_find(tab, c), c, [&](const float (&v)[8], long) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s[k & 1] = fma((double)v[k], (double)v[k], s[k & 1]);
+        }, [&](float v, long) { s[0] = fma((double)v, (double)v, s[0]); });
+    return s[0] + s[1];
 }
 
-// the norm and the factor from the partials: the same sum in the same order in every workgroup that asks for it
-__device__ __forceinline__ double clip_factor(const double* __restrict__ part, int parts, double max_norm, double scale, double* red, float* norm) {
-    double s = 0.0;
-    for (int i = threadIdx.x; i < parts; i += 256) s += part[i];
-    const double n = sqrt(clip_block_sum(s, red)) * fabs(scale);
+template <int THREADS>
+__device__ __forceinline__ void clip_scale(const ClipTab& tab, int first, int step, double f) {
+    // the last chunks first: they are what the norm's walk has left in the memory-side cache
+    for (int c = tab.chunk0[tab.count] - 1 - first; c >= 0; c -= step) {
+        const int t = clip_find(tab, c);
+        clip_walk<THREADS>(tab, t, c, [&](const float (&v)[8], long i) {
+            float o[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) o[k] = (float)((double)v[k] * f);
+            clip_st8(tab.out[t], i, tab.odt[t], o);
+        }, [&](float v, long i) { clip_st(tab.out[t], i, tab.odt[t], (float)((double)v * f)); });
+    }
+}
+
+// norm and factor from the sum of squares
+__device__ __forceinline__ double clip_factor(double sum, double max_norm, double scale, float* norm) {
+    const double n = sqrt(sum) * fabs(scale);
     if (norm && threadIdx.x == 0) *norm = (float)n;
     const double c = max_norm / (n + 1e-6);
     return (c > 1.0 ? 1.0 : c) * scale;                     // (a NaN norm stays one: every gradient becomes NaN)
 }
 
+__global__ __launch_bounds__(256) void clip_norm_kernel(const ClipTab tab, double* __restrict__ part) {
+    __shared__ double red[4];
+    const double s = clip_block_sum<256>(clip_squares<256>(tab, blockIdx.x, gridDim.x), red);
+    if (threadIdx.x == 0) part[blockIdx.x] = s;
+}
+
+// the partials' sum, the same in the same order in every workgroup that asks for it
+__device__ __forceinline__ double clip_total(const double* __restrict__ part, int parts, double* red) {
+    double s = 0.0;
+    for (int i = threadIdx.x; i < parts; i += 256) s += part[i];
+    return clip_block_sum<256>(s, red);
+}
+
 __global__ __launch_bounds__(256) void clip_scale_kernel(const ClipTab tab, const double* __restrict__ part, int parts, double max_norm, double scale,
                                                          float* __restrict__ norm, int in_place) {
     __shared__ double red[4];
-    const double f = clip_factor(part, parts, max_norm, scale, red, blockIdx.x == 0 ? norm : nullptr);
+    const double f = clip_factor(clip_total(part, parts, red), max_norm, scale, blockIdx.x == 0 ? norm : nullptr);
     if (in_place && f == 1.0) return;
-    const int total = tab.chunk0[tab.count];
-    for (int c = blockIdx.x; c < total; c += gridDim.x) {
-        const int t = clip_find(tab, c);
-        const long base = (long)(c - tab.chunk0[t]) * CLIP_CHUNK, end = min(tab.n[t], base + CLIP_CHUNK);
-        for (long i = base + threadIdx.x; i < end; i += 256) clip_st(tab.out[t], i, tab.odt[t], (float)((double)clip_ld(tab.g[t], i, tab.gdt[t]) * f));
-    }
+    clip_scale<256>(tab, blockIdx.x, gridDim.x, f);
 }
 
 __global__ __launch_bounds__(256) void clip_finish_kernel(const double* __restrict__ part, int parts, double scale, float* __restrict__ norm) {
     __shared__ double red[4];
-    clip_factor(part, parts, 1.0, scale, red, norm);
+    clip_factor(clip_total(part, parts, red), 1.0, scale, norm);
+}
+
+// Few elements: one workgroup does both in one launch (a second launch costs more than reading them again out of the cache)
+__global__ __launch_bounds__(1024) void clip_small_kernel(const ClipTab tab, double max_norm, double scale, float* __restrict__ norm, int want, int in_place) {
+    __shared__ double red[16];
+    const double f = clip_factor(clip_block_sum<1024>(clip_squares<1024>(tab, 0, 1), red), max_norm, scale, norm);
+    if (!want || (in_place && f == 1.0)) return;
+    clip_scale<1024>(tab, 0, 1, f);
 }
 
 int clip_fill(ClipTab& tab, int lo, int hi, const void* const* g, void* const* out, const int64_t* n, const int* gdt, const int* odt) {
@@ -124,6 +205,12 @@ extern "C" int sgg_clip_grads(const void* const* g, void* const* out, const int6
     hipStream_t s = (hipStream_t)stream;
     int parts = 0;
     ClipTab tab;
+    if (count <= CLIP_TAB && chunks_all <= CLIP_SMALL) {
+        clip_fill(tab, 0, count, g, out, n, g_dtype, out_dtype);
+        hipLaunchKernelGGL(clip_small_kernel, dim3(1), dim3(1024), 0, s, tab, max_norm, grad_scale, norm, out != nullptr, in_place);
+        SGG_CHECK_LAUNCH();
+        return SGG_OK;
+    }
     for (int lo = 0; lo < count; lo += CLIP_TAB) {
         const int chunks = clip_fill(tab, lo, min(count, lo + CLIP_TAB), g, out, n, g_dtype, out_dtype);
         if (!chunks) continue;

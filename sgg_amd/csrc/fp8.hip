@@ -164,44 +164,223 @@ __device__ __forceinline__ void mma_wide(f32x16& acc, const Wide& w, const Wide&
     for (int c = 0; c < 4; ++c) acc = mfma_32x32x16<SGG_BF16>(w.c[c], a.c[c], acc);
 }
 
+// ---- where results go: fp32 partial outputs of a K slice ([slice][M][N]), or act(sum + bias) in the output's type
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+
 __device__ __forceinline__ void out_st(char* C, long at, int dt, float v) {
     if (dt == SGG_F32) reinterpret_cast<float*>(C)[at] = v;
     else if (dt == SGG_BF16) reinterpret_cast<bf16_t*>(C)[at] = f32_to_bf16(v);
     else reinterpret_cast<f16_t*>(C)[at] = (f16_t)v;
 }
 
-// the plain tile: 128 x 128 outputs, 4 waves of 64 x 64, one block of 128 per step through LDS (2 x 16 KiB), rows past the end clamped
-template <bool WIDE>
-__global__ __launch_bounds__(256) void fp8_gemm_kernel(const Fp8Args g) {
-    __shared__ __attribute__((aligned(16))) unsigned char sA[128 * 128], sW[128 * 128];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int tilesN = (g.N + 127) / 128;
-    const long tm = blockIdx.x / tilesN, tn = blockIdx.x - tm * tilesN;
-    const long m0 = tm * 128, n0 = tn * 128;
-    const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64, fr = lane & 31, fh = lane >> 5;
-    const long blocks = g.Kp / 128, gA = ((long)g.M + 127) / 128, gW = ((long)g.N + 127) / 128;
-    f32x16 acc[2][2] = {};
-    for (long b = 0; b < blocks; ++b) {
-        __syncthreads();
+// 8 consecutive outputs of a row, nv of them inside (any alignment: this chip's 16-byte stores need none)
+__device__ __forceinline__ void out_row8(const Fp8Args& g, const float (&bias8)[8], float (&v)[8], long m, long n, int nv, float* part) {
+    if (part) {
+        float* o = part + m * g.N + n;
+        if (nv == 8) {
+            *reinterpret_cast<f32x4_any*>(o) = f32x4{v[0], v[1], v[2], v[3]};
+            *reinterpret_cast<f32x4_any*>(o + 4) = f32x4{v[4], v[5], v[6], v[7]};
+        } else {
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {                      // 128 rows of 8 16-byte pieces; pieces permuted by the row
-            const int r = p * 32 + (tid >> 3), h = tid & 7, at = r * 128 + ((h ^ (r & 7)) << 4);
-            *reinterpret_cast<u32x4*>(sA + at) = *reinterpret_cast<const u32x4*>(g.A + min(m0 + r, (long)g.M - 1) * g.Kp + b * 128 + h * 16);
-            *reinterpret_cast<u32x4*>(sW + at) = *reinterpret_cast<const u32x4*>(g.W + min(n0 + r, (long)g.N - 1) * g.Kp + b * 128 + h * 16);
+            for (int k = 0; k < 8; ++k)
+                if (k < nv) o[k] = v[k];
         }
-        __syncthreads();
-        const unsigned ea = reinterpret_cast<const unsigned*>(g.As)[(b * gA + tm) * 32 + fr] >> (wm / 4);
-        const unsigned ew = reinterpret_cast<const unsigned*>(g.Ws)[(b * gW + tn) * 32 + fr] >> (wn / 4);
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        v[k] += bias8[k];
+        if (g.act == SGG_ACT_RELU) v[k] = v[k] < 0.f ? 0.f : v[k];                       // (keeps NaN)
+    }
+    const long at = m * g.ldc + n;
+    if (nv < 8) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < nv) out_st(g.C, at + k, g.out_dt, v[k]);
+    } else if (g.out_dt == SGG_F32) {
+        float* o = reinterpret_cast<float*>(g.C) + at;
+        *reinterpret_cast<f32x4_any*>(o) = f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4_any*>(o + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    } else {
+        *reinterpret_cast<u32x4_any*>(g.C + at * 2) = g.out_dt == SGG_BF16 ? pack8<bf16_t>(v) : pack8<f16_t>(v);
+    }
+}
+
+// a wave's 32 MI x 64 outputs, from fragments whose lanes hold one row m and 4 consecutive n per register quad, to rows of 8 consecutive n per lane
+// through 8.5 KiB of LDS of its own (est; row stride 272 bytes)
+constexpr int EST = 32 * 272;
+template <int MI>
+__device__ __forceinline__ void out_wave(const Fp8Args& g, f32x16 (&acc)[MI][2], char* est, long m0, long n0, float* part) {
+    const int lane = threadIdx.x & 63, fr = lane & 31, fh = lane >> 5, rl = lane >> 3, cl = (lane & 7) * 8;
+    const long n = n0 + cl;
+    const int nv = (int)min(8L, max(0L, (long)g.N - n));
+    float bias8[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) bias8[k] = g.bias && !part && k < nv ? g.bias[n + k] : 0.f;
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi) {
+#pragma unroll
+        for (int ni = 0; ni < 2; ++ni)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                *reinterpret_cast<f32x4*>(est + fr * 272 + (ni * 32 + 8 * c + 4 * fh) * 4) =
+                    f32x4{acc[mi][ni][4 * c], acc[mi][ni][4 * c + 1], acc[mi][ni][4 * c + 2], acc[mi][ni][4 * c + 3]};
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                               // (its own writes: no other wave reads them)
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+            const long m = m0 + mi * 32 + rl + 8 * it;
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(est + (rl + 8 * it) * 272 + cl * 4);
+            const f32x4 hi = *reinterpret_cast<const f32x4*>(est + (rl + 8 * it) * 272 + cl * 4 + 16);
+            float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+            if (m < g.M && nv > 0) out_row8(g, bias8, v, m, n, nv, part);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+}
+
+// the K slices' partial outputs, added in slice order; then bias, activation and the output's rounding
+__global__ __launch_bounds__(256) void fp8_join_kernel(const Fp8Args g, const float* __restrict__ ws, int slices) {
+    const long n = ((long)blockIdx.x * 64 + (threadIdx.x & 63)) * 8;
+    if (n >= g.N) return;
+    const int nv = (int)min(8L, (long)g.N - n);
+    float bias8[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) bias8[k] = g.bias && k < nv ? g.bias[n + k] : 0.f;
+    for (long m = (long)blockIdx.y * 4 + (threadIdx.x >> 6); m < g.M; m += (long)gridDim.y * 4) {
+        float v[8] = {};
+        const float* p = ws + m * g.N + n;
+#pragma unroll 4
+        for (int s = 0; s < slices; ++s, p += (long)g.M * g.N) {
+            if (nv == 8) {
+                const f32x4 a = *reinterpret_cast<const f32x4_any*>(p), b = *reinterpret_cast<const f32x4_any*>(p + 4);
+                v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w; v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (k < nv) v[k] += p[k];
+            }
+        }
+        out_row8(g, bias8, v, m, n, nv, nullptr);
+    }
+}
+
+// ---- (1) up to 32 rows of A: a stream of W.  Bound by reading W once (its bytes / the memory's rate); everything else hides behind that.  A workgroup
+// owns 32 rows of W and a K slice, its 4 waves take the slice's blocks in turn (four neighbouring 128-byte pieces of every row are in flight together)
+// straight into registers, DEPTH blocks ahead of their use; the waves' sums meet in LDS.  Always the bf16 pipe: the conversions are a tenth of the
+// time W takes to arrive.
+template <int DEPTH>
+__global__ __launch_bounds__(256) void fp8_few_rows_kernel(const Fp8Args g, float* __restrict__ ws, int per) {
+    __shared__ float red[4][32 * 33];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 31, fh = lane >> 5;
+    const long n0 = (long)blockIdx.x * 32;
+    const int blocks = (int)(g.Kp / 128), b0 = min((int)blockIdx.y * per, blocks), b1 = min(b0 + per, blocks);
+    const long gA = ((long)g.M + 127) / 128, gW = ((long)g.N + 127) / 128;
+    const unsigned char* wp = g.W + min(n0 + fr, (long)g.N - 1) * g.Kp + fh * 16;
+    const unsigned char* ap = g.A + (long)min(fr, g.M - 1) * g.Kp + fh * 16;
+    const unsigned* sw = reinterpret_cast<const unsigned*>(g.Ws) + (n0 >> 7) * 32 + fr;
+    const unsigned* sa = reinterpret_cast<const unsigned*>(g.As) + fr;
+    const int shift = (int)(n0 >> 5 & 3) * 8;
+    struct { u32x4 w[4], a[4]; unsigned ew, ea; } buf[DEPTH];
+    auto fetch = [&](auto& t, int b) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) t.w[c] = *reinterpret_cast<const u32x4*>(wp + (long)b * 128 + c * 32);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) t.a[c] = *reinterpret_cast<const u32x4*>(ap + (long)b * 128 + c * 32);
+        t.ew = sw[(long)b * gW * 32];
+        t.ea = sa[(long)b * gA * 32];
+    };
+    f32x16 acc = {};
+#pragma unroll
+    for (int u = 0; u < DEPTH; ++u)
+        if (b0 + wave + 4 * u < b1) fetch(buf[u], b0 + wave + 4 * u);
+    for (int b = b0 + wave; b < b1; b += 4 * DEPTH) {
+#pragma unroll
+        for (int u = 0; u < DEPTH; ++u) {
+            if (b + 4 * u >= b1) continue;
+            const float fw = scale_f32<0>(buf[u].ew >> shift), fa = scale_f32<0>(buf[u].ea);
+            mma_wide(acc, widen(join8(buf[u].w[0], buf[u].w[1]), fw), widen(join8(buf[u].a[0], buf[u].a[1]), fa));
+            mma_wide(acc, widen(join8(buf[u].w[2], buf[u].w[3]), fw), widen(join8(buf[u].a[2], buf[u].a[3]), fa));
+            if (b + 4 * (u + DEPTH) < b1) fetch(buf[u], b + 4 * (u + DEPTH));
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) red[wave][fr * 33 + 8 * (r >> 2) + 4 * fh + (r & 3)] = acc[r];
+    __syncthreads();
+    float* part = gridDim.y > 1 ? ws + (long)blockIdx.y * g.M * g.N : nullptr;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int m = i * 8 + (tid >> 5);
+        const long n = n0 + (tid & 31);
+        if (m >= g.M || n >= g.N) continue;
+        const int at = m * 33 + (tid & 31);
+        float v = (red[0][at] + red[1][at]) + (red[2][at] + red[3][at]);
+        if (part) {
+            part[(long)m * g.N + n] = v;
+        } else {
+            v += g.bias ? g.bias[n] : 0.f;
+            out_st(g.C, m * g.ldc + n, g.out_dt, g.act == SGG_ACT_RELU && v < 0.f ? 0.f : v);
+        }
+    }
+}
+
+// ---- (2) the middle: tiles of 128 x 128, 4 waves of 64 x 64, one block of 128 per step, K slices while the tiles do not fill the chip.  Two LDS buffers
+// of 32 KiB (two workgroups per CU): while one block is multiplied, the next one's loads are in flight to registers.
+template <bool WIDE>
+__global__ __launch_bounds__(256) void fp8_tile_kernel(const Fp8Args g, float* __restrict__ ws, int per) {
+    __shared__ __attribute__((aligned(16))) unsigned char sm[2][2][128 * 128];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int tm, tn;
+    tile_coords(blockIdx.x, (g.M + 127) / 128, (g.N + 127) / 128, tm, tn);
+    const long m0 = (long)tm * 128, n0 = (long)tn * 128;
+    const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64, fr = lane & 31, fh = lane >> 5;
+    const int blocks = (int)(g.Kp / 128), b0 = min((int)blockIdx.y * per, blocks), b1 = min(b0 + per, blocks);
+    const long gA = ((long)g.M + 127) / 128, gW = ((long)g.N + 127) / 128;
+    const unsigned *sa = reinterpret_cast<const unsigned*>(g.As) + (long)tm * 32 + fr, *sw = reinterpret_cast<const unsigned*>(g.Ws) + (long)tn * 32 + fr;
+    // thread -> rows tid / 8 + 32 p, 16-byte piece tid % 8, stored at the piece permuted by the row (reads of 32 rows then spread over the banks)
+    const unsigned char *ap[4], *wp[4];
+    int at[4];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        const int r = p * 32 + (tid >> 3), h = tid & 7;
+        ap[p] = g.A + min(m0 + r, (long)g.M - 1) * g.Kp + h * 16;
+        wp[p] = g.W + min(n0 + r, (long)g.N - 1) * g.Kp + h * 16;
+        at[p] = r * 128 + ((h ^ (r & 7)) << 4);
+    }
+    u32x4 ra[4], rw[4];
+    unsigned ea_n = 0, ew_n = 0;
+    auto fetch = [&](int b) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            ra[p] = *reinterpret_cast<const u32x4*>(ap[p] + (long)b * 128);
+            rw[p] = *reinterpret_cast<const u32x4*>(wp[p] + (long)b * 128);
+        }
+        ea_n = sa[(long)b * gA * 32];
+        ew_n = sw[(long)b * gW * 32];
+    };
+    f32x16 acc[2][2] = {};
+    if (b0 < b1) fetch(b0);
+    for (int b = b0; b < b1; ++b) {
+        unsigned char *sA = sm[b & 1][0], *sW = sm[b & 1][1];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            *reinterpret_cast<u32x4*>(sA + at[p]) = ra[p];
+            *reinterpret_cast<u32x4*>(sW + at[p]) = rw[p];
+        }
+        const unsigned ea = ea_n >> (wm / 4), ew = ew_n >> (wn / 4);
+        if (b + 1 < b1) fetch(b + 1);
+        // one barrier per block: this buffer's last readers (block b - 2) passed the barrier of block b - 1 with their reads done
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             i32x8 a[2], w[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int ra = wm + i * 32 + fr, rw = wn + i * 32 + fr, h = s * 4 + fh * 2;
-                const u32x4 a0 = *reinterpret_cast<const u32x4*>(sA + ra * 128 + ((h ^ (ra & 7)) << 4)), a1 = *reinterpret_cast<const u32x4*>(sA + ra * 128 + (((h + 1) ^ (ra & 7)) << 4));
-                const u32x4 w0 = *reinterpret_cast<const u32x4*>(sW + rw * 128 + ((h ^ (rw & 7)) << 4)), w1 = *reinterpret_cast<const u32x4*>(sW + rw * 128 + (((h + 1) ^ (rw & 7)) << 4));
-                a[i] = join8(a0, a1);
-                w[i] = join8(w0, w1);
+                const int ra_ = wm + i * 32 + fr, rw_ = wn + i * 32 + fr, h = s * 4 + fh * 2;
+                a[i] = join8(*reinterpret_cast<const u32x4*>(sA + ra_ * 128 + ((h ^ (ra_ & 7)) << 4)), *reinterpret_cast<const u32x4*>(sA + ra_ * 128 + (((h + 1) ^ (ra_ & 7)) << 4)));
+                w[i] = join8(*reinterpret_cast<const u32x4*>(sW + rw_ * 128 + ((h ^ (rw_ & 7)) << 4)), *reinterpret_cast<const u32x4*>(sW + rw_ * 128 + (((h + 1) ^ (rw_ & 7)) << 4)));
             }
             if constexpr (WIDE) {
                 const Wide a0 = widen(a[0], scale_f32<0>(ea)), a1 = widen(a[1], scale_f32<1>(ea)), w0 = widen(w[0], scale_f32<0>(ew)), w1 = widen(w[1], scale_f32<1>(ew));
@@ -217,21 +396,222 @@ __global__ __launch_bounds__(256) void fp8_gemm_kernel(const Fp8Args g) {
             }
         }
     }
+    __syncthreads();                                          // (the staging below lies over the operand buffers)
+    out_wave<2>(g, acc, reinterpret_cast<char*>(sm) + wave * EST, m0 + wm, n0 + wn, gridDim.y > 1 ? ws + (long)blockIdx.y * g.M * g.N : nullptr);
+}
+
+// ---- (3) large: tiles of 256 x 256, 8 waves = two groups of four, one wave of each group per SIMD; a wave owns 128 x 64.  K advances in slabs of 64 bytes
+// per row (half a block).  The groups run the same slabs one phase apart, one barrier per phase: while one group's waves read their fragments of a slab
+// from LDS (and, for fp32 outputs, widen them), the other group's waves hold the matrix pipe:
+//   slot      0        1        2        3        4   ...
+//   group 0   LOAD 0   MFMA 0   LOAD 1   MFMA 1   LOAD 2
+//   group 1   -        LOAD 0   MFMA 0   LOAD 1   MFMA 1
+// A ring of 4 slabs (4 x 32 KiB) is filled by loads straight to LDS, three slabs ahead, issued between the matrix instructions and counted (never
+// drained before the end).  With a block's first slab travels the wave's own 256 bytes of scales: 32 dwords of its 128 rows of A, 32 of its rows of W.
+// 16-byte pieces of a row are permuted by (row / 4) % 4 on the source address and on the read: fragment reads of 32 rows hit every bank once.
+// one piece: uniform base + lane offset + immediate.  (The empty asm keeps the offset's widening next to the load, where it folds into the instruction's
+// scalar-base form; widened outside the loop it would be a 64-bit vector add per piece.  `off` is the caller's own variable: a copy's register
+// would be written again while the load is in flight, and the compiler waits for every load before that.)
+template <int OFF>
+__device__ __forceinline__ void lds_piece(const char* ubase, unsigned& off, char* l) {
+    asm volatile("" : "+v"(off));
+    __builtin_amdgcn_global_load_lds((glb_void_t*)(ubase + off), (lds_void_t*)l, 16, OFF, 0);
+}
+
+constexpr int PP_ROW = 64, PP_STAGE = 512 * PP_ROW, PP_RING = 4 * PP_STAGE, PP_SMEM = PP_RING + 4 * 8 * 256;
+
+template <bool WIDE>
+__global__ __launch_bounds__(512) void fp8_pingpong_kernel(const Fp8Args g, float* __restrict__ ws, int per) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int grp = wave >> 2, q = wave & 3, fr = lane & 31, fh = lane >> 5;
+    int tm, tn;
+    tile_coords(blockIdx.x, (g.M + 255) / 256, (g.N + 255) / 256, tm, tn);
+    const long m0 = (long)tm * 256, n0 = (long)tn * 256;
+    const int blocks = (int)(g.Kp / 128), b0 = min((int)blockIdx.y * per, blocks), b1 = min(b0 + per, blocks);
+    const int kb = 2 * b0, nt = 2 * b1;                       // slabs of this slice
+
+    // ---- loads to LDS: waves 0-3 the rows of A, waves 4-7 those of W; 4 instructions of 16 rows.  Global address = uniform base + a lane offset that
+    // never changes + the instruction's immediate, which also moves the LDS address: piece j lands j KiB behind ONE base (the lane offset carries
+    // -j KiB, and 3 KiB that the uniform base gives back keep it unsigned)
+    const bool loads_a = wave < 4;
+    const char* base = reinterpret_cast<const char*>(loads_a ? g.A + m0 * g.Kp : g.W + n0 * g.Kp);
+    unsigned vo[4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const long m = m0 + wm + i * 32 + fr;
-        if (m >= g.M) continue;
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const long n = n0 + wn + j * 32 + 8 * (r >> 2) + 4 * fh + (r & 3);
-                if (n >= g.N) continue;
-                float t = acc[i][j][r] + (g.bias ? g.bias[n] : 0.f);
-                if (g.act == SGG_ACT_RELU) t = t < 0.f ? 0.f : t;                         // (keeps NaN)
-                out_st(g.C, m * g.ldc + n, g.out_dt, t);
-            }
+    for (int j = 0; j < 4; ++j) {
+        const int r = (wave & 3) * 64 + j * 16 + (lane >> 2);
+        const long row = loads_a ? min(m0 + r, (long)g.M - 1) - m0 : min(n0 + r, (long)g.N - 1) - n0;        // (rows past the end: the last one again)
+        vo[j] = (unsigned)(row * g.Kp) + ((lane & 3) ^ ((r >> 2) & 3)) * 16 + 3072u - 1024u * j;
     }
+    unsigned vo_0 = vo[0], vo_1 = vo[1], vo_2 = vo[2], vo_3 = vo[3];
+    const int lds_rows0 = (loads_a ? 0 : 256 * PP_ROW) + (wave & 3) * 64 * PP_ROW;
+    const long gA = ((long)g.M + 127) / 128, gW = ((long)g.N + 127) / 128;
+    const unsigned* sp = lane < 32 ? reinterpret_cast<const unsigned*>(g.As) + ((long)b0 * gA + min((long)tm * 2 + grp, gA - 1)) * 32 + fr
+                                   : reinterpret_cast<const unsigned*>(g.Ws) + ((long)b0 * gW + min((long)tn * 2 + (q >> 1), gW - 1)) * 32 + fr;
+    const long sstep = (lane < 32 ? gA : gW) * 32;
+    char* const sreg = smem + PP_RING + wave * 256;
+    int sblock = b0;
+    // slabs are requested in order: kb .. nt - 1, then the last one three times more (into slabs of the ring that nobody reads again: the loop needs no tail)
+    auto issue_scales = [&](int kt) {                         // with each even slab
+        __builtin_amdgcn_global_load_lds((glb_void_t*)sp, (lds_void_t*)(sreg + ((kt >> 1) & 3) * 2048), 4, 0, 0);
+        if (++sblock < b1) sp += sstep;
+    };
+    auto slab_base = [&](int kt) { return uniform_ptr(base + (long)min(kt, nt - 1) * PP_ROW - 3072); };
+    auto issue = [&](int kt) {
+        const char* ub = slab_base(kt);
+        char* dst = smem + (kt & 3) * PP_STAGE + lds_rows0;
+        if (!(kt & 1)) issue_scales(kt);
+        lds_piece<0>(ub, vo_0, dst);
+        lds_piece<1024>(ub, vo_1, dst);
+        lds_piece<2048>(ub, vo_2, dst);
+        lds_piece<3072>(ub, vo_3, dst);
+    };
+
+    // LDS byte addresses of the lane's pieces fh and fh + 2 in slab 0: its first row of A and of W (the others 32 rows = 2 KiB further, same permutation)
+    const unsigned lds0 = (unsigned)(unsigned long)(lds_void_t*)smem;
+    const unsigned row_a = grp * 128 + fr, row_w = 256 + q * 64 + fr;
+    const unsigned at_a = lds0 + row_a * PP_ROW + ((fh ^ ((row_a >> 2) & 3)) << 4), at_w = lds0 + row_w * PP_ROW + ((fh ^ ((row_w >> 2) & 3)) << 4);
+    const unsigned at_s = lds0 + PP_RING + wave * 256 + fr * 4;
+    f32x16 acc[4][2] = {};
+    i32x8 af[4], wf[2];
+    Wide aw[4], ww[2];
+    unsigned ea = 0, ew = 0;
+    auto load_frags = [&](int kt, bool even) {
+        // one asm block, with its wait: the compiler waits for EVERY load to LDS in flight before an LDS read of its own
+        const unsigned st = (kt & 3) * PP_STAGE;
+        const unsigned a0 = at_a + st, a1 = a0 ^ 32, w0 = at_w + st, w1 = w0 ^ 32;
+        u32x4 f[12];
+#define FP8_READS                                                                                                              \
+    "ds_read_b128 %0, %14\n ds_read_b128 %1, %15\n ds_read_b128 %2, %14 offset:2048\n ds_read_b128 %3, %15 offset:2048\n"      \
+    "ds_read_b128 %4, %12\n ds_read_b128 %5, %13\n ds_read_b128 %6, %12 offset:2048\n ds_read_b128 %7, %13 offset:2048\n"      \
+    "ds_read_b128 %8, %12 offset:4096\n ds_read_b128 %9, %13 offset:4096\n ds_read_b128 %10, %12 offset:6144\n ds_read_b128 %11, %13 offset:6144\n"
+        asm volatile(FP8_READS "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(f[0]), "=&v"(f[1]), "=&v"(f[2]), "=&v"(f[3]), "=&v"(f[4]), "=&v"(f[5]), "=&v"(f[6]), "=&v"(f[7]), "=&v"(f[8]), "=&v"(f[9]), "=&v"(f[10]), "=&v"(f[11])
+                     : "v"(a0), "v"(a1), "v"(w0), "v"(w1)
+                     : "memory");
+#undef FP8_READS
+        if (even) {
+            unsigned e;
+            asm volatile("ds_read_b32 %0, %2\n ds_read_b32 %1, %2 offset:128\n s_waitcnt lgkmcnt(0)" : "=&v"(ea), "=&v"(e) : "v"(at_s + ((kt >> 1) & 3) * 2048) : "memory");
+            ew = e >> ((q & 1) * 16);
+        }
+        wf[0] = join8(f[0], f[1]); wf[1] = join8(f[2], f[3]);
+        af[0] = join8(f[4], f[5]); af[1] = join8(f[6], f[7]); af[2] = join8(f[8], f[9]); af[3] = join8(f[10], f[11]);
+        if constexpr (WIDE) {
+            ww[0] = widen(wf[0], scale_f32<0>(ew)); ww[1] = widen(wf[1], scale_f32<1>(ew));
+            aw[0] = widen(af[0], scale_f32<0>(ea)); aw[1] = widen(af[1], scale_f32<1>(ea));
+            aw[2] = widen(af[2], scale_f32<2>(ea)); aw[3] = widen(af[3], scale_f32<3>(ea));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+#define FP8_MMA(mi)                                                                                                                              \
+    if constexpr (WIDE) {                                                                                                                        \
+        mma_wide(acc[mi][0], ww[0], aw[mi]);                                                                                                     \
+        mma_wide(acc[mi][1], ww[1], aw[mi]);                                                                                                     \
+    } else {                                                                                                                                     \
+        acc[mi][0] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[0], af[mi], acc[mi][0], 0, 0, 0, ew, mi, ea);                             \
+        acc[mi][1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[1], af[mi], acc[mi][1], 0, 0, 1, ew, mi, ea);                             \
+    }
+    auto compute_dma = [&](int pf, bool scales) {             // the slab's matrix instructions with the loads of slab pf between them
+        const char* ub = slab_base(pf);
+        char* dst = smem + (pf & 3) * PP_STAGE + lds_rows0;
+        if (scales) issue_scales(pf);
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(1);
+        FP8_MMA(0)
+        lds_piece<0>(ub, vo_0, dst);
+        __builtin_amdgcn_sched_barrier(0);
+        FP8_MMA(1)
+        lds_piece<1024>(ub, vo_1, dst);
+        __builtin_amdgcn_sched_barrier(0);
+        FP8_MMA(2)
+        lds_piece<2048>(ub, vo_2, dst);
+        __builtin_amdgcn_sched_barrier(0);
+        FP8_MMA(3)
+        lds_piece<3072>(ub, vo_3, dst);
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+#undef FP8_MMA
+#define FP8_BARRIER()                     \
+    {                                     \
+        __builtin_amdgcn_s_barrier();     \
+        asm volatile("" ::: "memory");    \
+        __builtin_amdgcn_sched_barrier(0);\
+    }
+    // Waits.  A wave issues 5 loads with an even slab (scales first), 4 with an odd one, slabs in order.  Before the barrier behind which slab kt + 1 is
+    // read, a wave may still have in flight what it issued after slab kt + 1: group 0 (at the end of MFMA kt, having issued kt + 3) slabs kt + 2 and
+    // kt + 3 = 9; group 1 (in LOAD kt, having issued kt + 2) that slab = 5 or 4.
+    issue(kb);
+    issue(kb + 1);
+    issue(kb + 2);
+    wait_vmcnt<9>();
+    FP8_BARRIER()
+    // slab kt + 3 goes where slab kt - 1 was: its last readers (group 1, LOAD kt - 1) had their reads done before the barrier that ended that phase
+    if (grp == 0) {
+        for (int kt = kb; kt < nt; kt += 2) {
+            load_frags(kt, true);
+            FP8_BARRIER()
+            compute_dma(kt + 3, false);
+            wait_vmcnt<9>();
+            FP8_BARRIER()
+            load_frags(kt + 1, false);
+            FP8_BARRIER()
+            compute_dma(kt + 4, true);
+            wait_vmcnt<9>();
+            FP8_BARRIER()
+        }
+        FP8_BARRIER()                                         // slot 2 nt: group 1's last MFMA phase
+    } else {
+        FP8_BARRIER()                                         // slot 0
+        for (int kt = kb; kt < nt; kt += 2) {
+            load_frags(kt, true);
+            wait_vmcnt<5>();
+            FP8_BARRIER()
+            compute_dma(kt + 3, false);
+            FP8_BARRIER()
+            load_frags(kt + 1, false);
+            wait_vmcnt<4>();
+            FP8_BARRIER()
+            compute_dma(kt + 4, true);
+            FP8_BARRIER()
+        }
+    }
+    wait_vmcnt<0>();                                          // (every load to LDS has landed before the staging below lies over the ring)
+    __syncthreads();
+    out_wave<4>(g, acc, smem + wave * EST, m0 + grp * 128, n0 + q * 64, gridDim.y > 1 ? ws + (long)blockIdx.y * g.M * g.N : nullptr);
+}
+
+// ---- which kernel and how many K slices
+enum { FP8_FEW, FP8_TILE, FP8_PINGPONG };
+struct Fp8Plan { int kernel, tiles, slices, per; };
+
+Fp8Plan fp8_plan(int64_t M, int64_t N, int64_t Kp) {
+    const int64_t blocks = Kp / 128, t128 = ((M + 127) / 128) * ((N + 127) / 128), t256 = ((M + 255) / 256) * ((N + 255) / 256);
+    int64_t kernel, tiles, want;
+    if (M <= 32) {
+        kernel = FP8_FEW;
+        tiles = (N + 31) / 32;
+        want = min(512 / max(tiles, (int64_t)1), blocks / 8);                 // two workgroups per CU, two blocks or more per wave
+    } else if (t256 >= 192 && blocks >= 1 && Kp <= (1 << 23)) {
+        kernel = FP8_PINGPONG;
+        tiles = t256;
+        want = 1;
+    } else {
+        kernel = FP8_TILE;
+        tiles = t128;
+        want = min(512 / max(tiles, (int64_t)1), blocks / 4);
+    }
+    const int64_t slices = max(want, (int64_t)1), per = max((blocks + slices - 1) / slices, (int64_t)1);
+    return {(int)kernel, tiles > 0x7fffffff ? -1 : (int)tiles, (int)max((blocks + per - 1) / per, (int64_t)1), (int)per};       // (no empty slice)
+}
+
+template <typename K>
+int fp8_launch(K kernel, const Fp8Plan& p, int threads, int smem, const Fp8Args& g, float* ws, hipStream_t s) {
+    if (smem > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, smem) != hipSuccess) return SGG_ERR_LAUNCH;
+    hipLaunchKernelGGL(kernel, dim3(p.tiles, p.slices), dim3(threads), smem, s, g, ws, p.per);
+    SGG_CHECK_LAUNCH();
+    return SGG_OK;
 }
 
 }  // namespace
@@ -260,24 +640,28 @@ extern "C" int sgg_fp8_quantize(const void* x, int64_t ldx, int64_t M, int64_t K
 
 // K slices of a product whose output tiles alone do not fill the chip; ws then holds that many fp32 [M][N] partial outputs
 extern "C" int sgg_gemm_fp8_splits(int64_t M, int64_t N, int64_t Kp) {
-    if (M < 0 || N < 0 || Kp < 0 || Kp % 128) return SGG_ERR_ARG;
-    return 1;
+    if (M < 0 || N < 0 || Kp < 0 || Kp % 128 || M > 0x7fffff00 || N > 0x7fffff00 || Kp > 0x7fffff00) return SGG_ERR_ARG;
+    return fp8_plan(M, N, Kp).slices;
 }
 
 extern "C" int sgg_gemm_fp8(const void* A, const void* A_scale, const void* W, const void* W_scale, const float* bias, void* C, int64_t ldc, int64_t M,
                             int64_t N, int64_t Kp, int act, int out_dtype, float* ws, void* stream) {
     if (!sgg_is_dtype(out_dtype)) return SGG_ERR_DTYPE;
-    if (M < 0 || N < 0 || Kp < 0 || Kp % 128 || M > 0x7fffff00 || N > 0x7fffff00 || ldc < N || (act != SGG_ACT_NONE && act != SGG_ACT_RELU)) return SGG_ERR_ARG;
+    if (M < 0 || N < 0 || Kp < 0 || Kp % 128 || M > 0x7fffff00 || N > 0x7fffff00 || Kp > 0x7fffff00 || ldc < N || (act != SGG_ACT_NONE && act != SGG_ACT_RELU))
+        return SGG_ERR_ARG;
     if (M == 0 || N == 0) return SGG_OK;
     if (!C || (Kp > 0 && (!A || !A_scale || !W || !W_scale)) || (((uintptr_t)A | (uintptr_t)W) & 15) || (((uintptr_t)A_scale | (uintptr_t)W_scale) & 3)) return SGG_ERR_ARG;
-    const int splits = sgg_gemm_fp8_splits(M, N, Kp);
-    if (splits > 1 && !ws) return SGG_ERR_ARG;
+    const Fp8Plan p = fp8_plan(M, N, Kp);
+    if (p.tiles < 0 || (p.slices > 1 && !ws)) return SGG_ERR_ARG;
     const Fp8Args g = {(const unsigned char*)A, (const unsigned char*)A_scale, (const unsigned char*)W, (const unsigned char*)W_scale, bias, (char*)C, (long)ldc, (long)Kp, (int)M, (int)N, act, out_dtype};
-    const int64_t tiles = ((M + 127) / 128) * ((N + 127) / 128);
-    if (tiles > 0x7fffffff) return SGG_ERR_ARG;
     hipStream_t s = (hipStream_t)stream;
-    if (out_dtype == SGG_F32) hipLaunchKernelGGL(fp8_gemm_kernel<true>, dim3((unsigned)tiles), dim3(256), 0, s, g);
-    else hipLaunchKernelGGL(fp8_gemm_kernel<false>, dim3((unsigned)tiles), dim3(256), 0, s, g);
+    const bool wide = out_dtype == SGG_F32;
+    int rc;
+    if (p.kernel == FP8_FEW) rc = fp8_launch(fp8_few_rows_kernel<4>, p, 256, 0, g, ws, s);
+    else if (p.kernel == FP8_TILE) rc = wide ? fp8_launch(fp8_tile_kernel<true>, p, 256, 0, g, ws, s) : fp8_launch(fp8_tile_kernel<false>, p, 256, 0, g, ws, s);
+    else rc = wide ? fp8_launch(fp8_pingpong_kernel<true>, p, 512, PP_SMEM, g, ws, s) : fp8_launch(fp8_pingpong_kernel<false>, p, 512, PP_SMEM, g, ws, s);
+    if (rc != SGG_OK || p.slices == 1) return rc;
+    hipLaunchKernelGGL(fp8_join_kernel, dim3((unsigned)((N + 511) / 512), (unsigned)min((M + 3) / 4, (int64_t)1024)), dim3(256), 0, s, g, ws, p.slices);
     SGG_CHECK_LAUNCH();
     return SGG_OK;
 }

@@ -334,7 +334,10 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Layer normalisation over the last axis of x [..., C] (f32 / bf16 / f16; statistics and sums in fp32) with weight, bias f32[C] or None
     -> x's shape and type; differentiable in all three (csrc/layernorm.hip: one pass each way)."""
     _need_gpu(x)
-    return _LayerNorm.apply(x.reshape(-1, x.shape[-1]), weight, bias, eps).view(x.shape)
+    rows = x.reshape(-1, x.shape[-1])
+    if not torch.is_grad_enabled():
+        return ops.layer_norm(_row_form(rows), weight, bias, eps, stats=False)[0].view(x.shape)
+    return _LayerNorm.apply(rows, weight, bias, eps).view(x.shape)
 
 
 class LayerNormRows(nn.LayerNorm):

@@ -3,6 +3,7 @@
 torch is used for device memory and the current HIP stream only; every wrapper hands raw device pointers
 to libsgg_hip.so.  Nothing here computes on the CPU and nothing falls back to torch ops.
 """
+import ctypes
 import os
 
 import torch
@@ -1172,12 +1173,15 @@ LAYER_NORM_MAX = 16384      # include/sgg_hip.h SGG_LAYER_NORM_MAX: widest row o
 FP8_BLOCK = 128             # columns that share a scale
 
 
+_current_device = getattr(torch._C, '_cuda_getDevice', None) or torch.cuda.current_device
+
+
 def _here(t, what):
     """the launch goes to the current device's stream: a tensor of another device is refused, not run there"""
-    if not t.is_cuda:
-        raise RuntimeError('sgg_amd: %s: tensor is not on the GPU (the HIP path has no CPU fallback)' % what)
-    if t.device.index != torch.cuda.current_device():
-        raise RuntimeError('sgg_amd: %s: tensor is on %s, the current device is cuda:%d' % (what, t.device, torch.cuda.current_device()))
+    if t.get_device() != _current_device():
+        if not t.is_cuda:
+            raise RuntimeError('sgg_amd: %s: tensor is not on the GPU (the HIP path has no CPU fallback)' % what)
+        raise RuntimeError('sgg_amd: %s: tensor is on %s, the current device is cuda:%d' % (what, t.device, _current_device()))
 
 
 def _row_matrix(t, what):
@@ -1316,38 +1320,41 @@ def _dense_layout(t):
 
 def _grad_list(grads, what):
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-    dev = torch.cuda.current_device() if grads else None
     for g in grads:
-        if not g.is_cuda or g.device.index != dev:
-            _here(g, what)
-        if g.layout != torch.strided:
+        _here(g, what)
+        if g.layout is not torch.strided:
             raise TypeError('sgg_amd: %s: dense gradients only (got %s)' % (what, g.layout))
     return grads
 
 
+def _tensor_table(ts):
+    """-> (addresses, sizes, type codes, [(start, end, type)] of the memory of each)"""
+    ptr = [t.data_ptr() for t in ts]
+    num = [t.numel() for t in ts]
+    code = [dt(t) for t in ts]
+    return ptr, num, code, [(p, p + n * (4 if c == SGG_F32 else 2), c) for p, n, c in zip(ptr, num, code)]
+
+
 def _clip_call(grads, outs, max_norm, grad_scale):
-    import numpy as np
     n = len(grads)
+    lib = _lib.load()
     norm = torch.empty((), dtype=torch.float32, device='cuda')
-    ws = torch.empty(_lib.load().sgg_clip_grads_parts(n), dtype=torch.float64, device='cuda')
-    gp = np.array([g.data_ptr() for g in grads], dtype=np.uint64)
-    nn = np.array([g.numel() for g in grads], dtype=np.int64)
-    gd = np.array([dt(g) for g in grads], dtype=np.int32)
-    op = od = None
+    ws = torch.empty(lib.sgg_clip_grads_parts(n), dtype=torch.float64, device='cuda')
+    ptr, num, code, mem = _tensor_table(grads)
+    optr, ocode = ptr, code
     if outs is not None:
-        op, od = (gp, gd) if outs is grads else (np.array([o.data_ptr() for o in outs], dtype=np.uint64), np.array([dt(o) for o in outs], dtype=np.int32))
         # every tensor is written by workgroups of its own: no two of them may share memory (one given twice would be scaled twice)
-        lo, hi = gp, gp + nn.astype(np.uint64) * np.where(gd == SGG_F32, 4, 2).astype(np.uint64)
-        if op is not gp:
-            apart = (op != gp) | (od != gd)
-            lo = np.concatenate((lo, op[apart]))
-            hi = np.concatenate((hi, (op + nn.astype(np.uint64) * np.where(od == SGG_F32, 4, 2).astype(np.uint64))[apart]))
-        order = np.argsort(lo[hi > lo], kind='stable')
-        a, b = lo[hi > lo][order], hi[hi > lo][order]
-        if (a[1:] < b[:-1]).any():
-            raise ValueError('sgg_amd: clip_grads_: two of the tensors share memory')
-    _lib.call('sgg_clip_grads', gp.ctypes.data, op.ctypes.data if op is not None else None, nn.ctypes.data, gd.ctypes.data,
-              od.ctypes.data if od is not None else None, n, float(max_norm), float(grad_scale), ws.data_ptr(), norm.data_ptr(), _stream())
+        if outs is not grads:
+            optr, _, ocode, omem = _tensor_table(outs)
+            mem = mem + [o for o, g in zip(omem, mem) if o != g]             # (an output that IS its gradient: in place)
+        mem = sorted(m for m in mem if m[1] > m[0])
+        for a, b in zip(mem, mem[1:]):
+            if b[0] < a[1]:
+                raise ValueError('sgg_amd: clip_grads_: two of the tensors share memory')
+    Ptrs, Longs, Ints = ctypes.c_void_p * n, ctypes.c_int64 * n, ctypes.c_int * n
+    g, d, sizes = Ptrs(*ptr), Ints(*code), Longs(*num)
+    o, od = (None, None) if outs is None else (g, d) if outs is grads else (Ptrs(*optr), Ints(*ocode))
+    _lib.call('sgg_clip_grads', g, o, sizes, d, od, n, float(max_norm), float(grad_scale), ws.data_ptr(), norm.data_ptr(), _stream())
     return norm
 
 
