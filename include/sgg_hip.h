@@ -22,7 +22,7 @@
 extern "C" {
 #endif
 
-#define SGG_ABI_VERSION 15   /* bump whenever a prototype below changes: tests/abi.lock pins (version, digest of the prototypes) */
+#define SGG_ABI_VERSION 16   /* bump whenever a prototype below changes: tests/abi.lock pins (version, digest of the prototypes) */
 
 enum { SGG_F32 = 0, SGG_BF16 = 1, SGG_F16 = 2,
        /* a PAIR of f16 planes x = hi + lo (hi = f16(x), lo = f16(x - hi): 22 significand bits) -- the operand / activation format of the x3
@@ -419,12 +419,14 @@ int sgg_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ldx
  * Operand form of x [M, K]: `rows` u8 [M][Kp], Kp = K rounded up to 128 (zeros past K), and rows_scale u8 [sgg_fp8_scale_bytes(M, K)]: the
  * exponent byte e + 127 of each row and block, e >= -126 the smallest with max|x| <= 448 * 2^e over the block's finite elements (non-finite
  * elements become NaN); byte ((b * G + m / 128) * 32 + m % 32) * 4 + (m / 32) % 4, G = ceil(M / 128).  `cols` / cols_scale: the same form of x^T
- * ([K][Mp]), out of the same reading of x.  Either form may be NULL (with its scales).  rows, cols 16-byte aligned.
+ * ([K][Mp]), out of the same reading of x.  Either form may be NULL (with its scales).  rows, cols 16-byte aligned, the scales 4-byte.
+ * colsum f32[K] (or NULL; only with `cols`): the column sums of x (a bias gradient of x = dY), added in a fixed order; colsum_ws
+ * f32[ceil(M / 128) * K] then.
  * gemm_fp8: C[m][n] = act(sum_k A[m][k] W[n][k] + bias[n]), fp32 accumulation, one rounding to out_dtype; bias f32[N] or NULL; ldc in
  * elements; ws f32[splits * M * N] when sgg_gemm_fp8_splits(M, N, Kp) is more than 1 (the K slices are added in a fixed order). */
 int64_t sgg_fp8_scale_bytes(int64_t rows, int64_t K);
-int sgg_fp8_quantize(const void* x, int64_t ldx, int64_t M, int64_t K, void* rows, void* rows_scale, void* cols, void* cols_scale, int dtype,
-                     void* stream);
+int sgg_fp8_quantize(const void* x, int64_t ldx, int64_t M, int64_t K, void* rows, void* rows_scale, void* cols, void* cols_scale, float* colsum,
+                     float* colsum_ws, int dtype, void* stream);
 int sgg_gemm_fp8_splits(int64_t M, int64_t N, int64_t Kp);
 int sgg_gemm_fp8(const void* A, const void* A_scale, const void* W, const void* W_scale, const float* bias, void* C, int64_t ldc, int64_t M, int64_t N,
                  int64_t Kp, int act, int out_dtype, float* ws, void* stream);

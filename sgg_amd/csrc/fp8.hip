@@ -17,99 +17,145 @@ constexpr int QB = 128;             // columns of a block
 __host__ __device__ __forceinline__ long scale_bytes(long rows, long blocks) { return blocks * ((rows + 127) / 128) * 128; }
 __device__ __forceinline__ long scale_at(long m, long blk, long groups) { return ((blk * groups + (m >> 7)) * 32 + (m & 31)) * 4 + ((m >> 5) & 3); }
 
-// biased exponent byte of the block whose largest finite magnitude has the bits `top`:  max = 1.f * 2^E; 448 = 1.75 * 2^8
-__device__ __forceinline__ int scale_byte(unsigned top) {
-    const int E = (int)(top >> 23);                                   // biased
-    return max(1, E - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0));
+// biased exponent byte of the block whose largest finite magnitude is `top`:  top = 1.f * 2^E; 448 = 1.75 * 2^8
+__device__ __forceinline__ int scale_byte(float top) {
+    const unsigned t = __float_as_uint(top);
+    return max(1, (int)(t >> 23) - 8 + ((t & 0x7fffffu) > 0x600000u ? 1 : 0));
 }
 __device__ __forceinline__ float scale_inv(int byte) { return __uint_as_float((unsigned)(254 - byte) << 23); }        // 2^-(byte - 127)
-__device__ __forceinline__ unsigned finite_bits(float v) {
-    const unsigned a = __float_as_uint(v) & 0x7fffffffu;
-    return a < 0x7f800000u ? a : 0u;
-}
-__device__ __forceinline__ float scaled(float v, float inv) {         // what the conversion is given: NaN for every non-finite input
-    return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u ? __uint_as_float(0x7fc00000u) : v * inv;
-}
+__device__ __forceinline__ bool is_inf(float v) { return (__float_as_uint(v) & 0x7fffffffu) == 0x7f800000u; }
+__device__ __forceinline__ float not_inf(float v) { return is_inf(v) ? 0.f : fabsf(v); }
 __device__ __forceinline__ unsigned pack_fp8x4(float a, float b, float c, float d) {
     int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
     return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
 }
+// 8 values times inv -> 8 codes; infinities go as NaN (a NaN stays one by itself)
+__device__ __forceinline__ u32x2 pack_fp8x8(const float (&v)[8], float inv, bool inf) {
+    float q[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = v[j] * inv;
+    if (inf) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] = is_inf(v[j]) ? __uint_as_float(0x7fc00000u) : q[j];
+    }
+    return u32x2{pack_fp8x4(q[0], q[1], q[2], q[3]), pack_fp8x4(q[4], q[5], q[6], q[7])};
+}
+// max over the 16 lanes of a DPP row (values >= 0)
+__device__ __forceinline__ float row16_max(float v) {
+#define FP8_DPP_MAX(ctrl) v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, 0xF, 0xF, false)));
+    FP8_DPP_MAX(0xB1)   // quad_perm [1,0,3,2]
+    FP8_DPP_MAX(0x4E)   // quad_perm [2,3,0,1]
+    FP8_DPP_MAX(0x141)  // row_half_mirror
+    FP8_DPP_MAX(0x140)  // row_mirror
+#undef FP8_DPP_MAX
+    return v;
+}
 
-// One workgroup = a tile of 128 x 128 values; thread (tr, tc) holds rows 8 tr .. 8 tr + 7, columns 8 tc .. 8 tc + 7.  The row form needs the
-// largest magnitude of each row of the tile (16 lanes meet), the transposed form that of each column (LDS), so both come from one reading.
-template <typename T, bool ROWS, bool COLS>
+// One workgroup = a tile of 128 x 128 values; thread (tr, tc) holds rows 8 tr .. 8 tr + 7, columns 8 tc .. 8 tc + 7.  The row form needs the largest
+// magnitude of each row of the tile (16 lanes meet), the transposed form that of each column (LDS), the column sums (a bias gradient) one number per
+// column: all out of one reading, which is what bounds it (8-byte and 16-byte stores, every line of both outputs written whole).
+// max() drops NaN, so only infinities need a second look: a tile's rows (columns) are gone over again without them where the maximum is infinite.
+template <typename T, bool ROWS, bool COLS, bool SUM>
 __global__ __launch_bounds__(256) void fp8_quantize_kernel(const T* __restrict__ x, long ldx, long M, int K, unsigned char* __restrict__ rows,
                                                            unsigned char* __restrict__ rscale, unsigned char* __restrict__ cols,
-                                                           unsigned char* __restrict__ cscale, int tilesM) {
-    __shared__ __attribute__((aligned(16))) unsigned char tile[128 * 128];
-    __shared__ unsigned cmax[16][128];
+                                                           unsigned char* __restrict__ cscale, float* __restrict__ sums, int tilesK) {
+    __shared__ __attribute__((aligned(16))) unsigned char tile[COLS ? 128 * 128 : 16];
+    __shared__ float cred[COLS ? 16 : 1][128];
+    __shared__ unsigned char rbyte[128], cbyte[128], cinf[128];
     const int tid = threadIdx.x, tr = tid >> 4, tc = tid & 15;
-    const int tk = blockIdx.x / tilesM;
-    const long tm = blockIdx.x - (long)tk * tilesM;
+    const long tm = blockIdx.x / tilesK;
+    const int tk = (int)(blockIdx.x - tm * tilesK);
     const long m0 = tm * 128;
     const int k0 = tk * QB;
     const long Kp = ((long)K + 127) / 128 * 128;
     float v[8][8];
-    const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ldx * (long)sizeof(T)) % 16 == 0;
+    const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ldx * (long)sizeof(T)) % 16 == 0 && k0 + tc * 8 + 8 <= K;
+    const T* p0 = x + (m0 + tr * 8) * ldx + k0 + tc * 8;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const long m = m0 + tr * 8 + i;
-        const int k = k0 + tc * 8;
-        const T* p = x + m * ldx + k;
-        if (m < M && vec && k + 8 <= K) {
-            load8(p, v[i]);
+        const bool in = m0 + tr * 8 + i < M;
+        if (in && vec) {
+            load8(p0 + i * ldx, v[i]);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = m < M && k + j < K ? Elem<T>::ld(p + j) : 0.f;
+            for (int j = 0; j < 8; ++j) v[i][j] = in && k0 + tc * 8 + j < K ? Elem<T>::ld(p0 + i * ldx + j) : 0.f;
         }
     }
     if constexpr (ROWS) {
-        const long groups = (M + 127) / 128;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            unsigned top = 0;
+            float top = 0.f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top = max(top, finite_bits(v[i][j]));
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[i][j]));
+            top = row16_max(top);
+            const bool inf = is_inf(top);
+            if (inf) {                                            // (all 16 lanes of the row together)
+                top = 0.f;
 #pragma unroll
-            for (int o = 8; o > 0; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o, 16));
-            const long m = m0 + tr * 8 + i;
+                for (int j = 0; j < 8; ++j) top = fmaxf(top, not_inf(v[i][j]));
+                top = row16_max(top);
+            }
             const int byte = scale_byte(top);
-            const float inv = scale_inv(byte);
-            float q[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) q[j] = scaled(v[i][j], inv);
-            if (m < M) *reinterpret_cast<u32x2*>(rows + m * Kp + k0 + tc * 8) = u32x2{pack_fp8x4(q[0], q[1], q[2], q[3]), pack_fp8x4(q[4], q[5], q[6], q[7])};
-            if (tc == 0) rscale[scale_at(m, tk, groups)] = (unsigned char)byte;          // (rows past M of the last group: blocks of zeros)
+            const long m = m0 + tr * 8 + i;
+            if (m < M) *reinterpret_cast<u32x2*>(rows + m * Kp + k0 + tc * 8) = pack_fp8x8(v[i], scale_inv(byte), inf);
+            if (tc == 0) rbyte[tr * 8 + i] = (unsigned char)byte;                        // (rows past M of the last group: blocks of zeros)
         }
     }
     if constexpr (COLS) {
-        const long Mp = (M + 127) / 128 * 128, groups = ((long)K + 127) / 128;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            unsigned top = 0;
+            float top = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) top = max(top, finite_bits(v[i][j]));
-            cmax[tr][tc * 8 + j] = top;
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i][j]));
+            cred[tr][tc * 8 + j] = top;
         }
-        __syncthreads();
+    }
+    if constexpr (ROWS || COLS) __syncthreads();
+    if constexpr (ROWS)
+        if (tid < 32) {
+            const long groups = (M + 127) / 128;
+            reinterpret_cast<unsigned*>(rscale)[((long)tk * groups + tm) * 32 + tid] =
+                rbyte[tid] | (unsigned)rbyte[tid + 32] << 8 | (unsigned)rbyte[tid + 64] << 16 | (unsigned)rbyte[tid + 96] << 24;
+        }
+    if constexpr (COLS) {
+        const long Mp = (M + 127) / 128 * 128, groups = ((long)K + 127) / 128;
         if (tid < 128) {
-            unsigned top = 0;
+            float top = 0.f;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) top = max(top, cmax[r][tid]);
-            const int byte = scale_byte(top);
-            cmax[0][tid] = (unsigned)byte;
-            cscale[scale_at(k0 + tid, tm, groups)] = (unsigned char)byte;
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, cred[r][tid]);
+            cinf[tid] = is_inf(top);
+            cbyte[tid] = (unsigned char)scale_byte(top);
         }
-        __syncthreads();
+        if (__syncthreads_or(tid < 128 && cinf[tid])) {           // some column holds an infinity: the columns' maxima again, without them
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float top = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, not_inf(v[i][j]));
+                cred[tr][tc * 8 + j] = top;
+            }
+            __syncthreads();
+            if (tid < 128) {
+                float top = 0.f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) top = fmaxf(top, cred[r][tid]);
+                cbyte[tid] = (unsigned char)scale_byte(top);
+            }
+            __syncthreads();
+        }
+        if (tid < 32)
+            reinterpret_cast<unsigned*>(cscale)[(tm * groups + tk) * 32 + tid] =
+                cbyte[tid] | (unsigned)cbyte[tid + 32] << 8 | (unsigned)cbyte[tid + 64] << 16 | (unsigned)cbyte[tid + 96] << 24;
         // transposed tile in LDS: column c's 128 bytes, their 8-byte pieces permuted by c / 8 so that neither side's accesses pile up on a bank
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int c = tc * 8 + j;
-            const float inv = scale_inv((int)cmax[0][c]);
-            float q[8];
+            const float t[8] = {v[0][j], v[1][j], v[2][j], v[3][j], v[4][j], v[5][j], v[6][j], v[7][j]};
+            *reinterpret_cast<u32x2*>(tile + c * 128 + ((tr ^ tc) << 3)) = pack_fp8x8(t, scale_inv(cbyte[c]), cinf[c]);
+        }
+        if constexpr (SUM) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) q[i] = scaled(v[i][j], inv);
-            *reinterpret_cast<u32x2*>(tile + c * 128 + ((tr ^ tc) << 3)) = u32x2{pack_fp8x4(q[0], q[1], q[2], q[3]), pack_fp8x4(q[4], q[5], q[6], q[7])};
+            for (int j = 0; j < 8; ++j) cred[tr][tc * 8 + j] = ((v[0][j] + v[1][j]) + (v[2][j] + v[3][j])) + ((v[4][j] + v[5][j]) + (v[6][j] + v[7][j]));
         }
         __syncthreads();
 #pragma unroll
@@ -119,6 +165,13 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(const T* __restrict__
             const u32x2 b = *reinterpret_cast<const u32x2*>(tile + c * 128 + (((2 * h + 1) ^ key) << 3));
             if (k0 + c < K) *reinterpret_cast<u32x4*>(cols + (long)(k0 + c) * Mp + m0 + h * 16) = u32x4{a.x, a.y, b.x, b.y};
         }
+        if constexpr (SUM)
+            if (tid < 128 && k0 + tid < K) {                      // this tile's 128 rows; the tiles' sums are added in order by the caller
+                float t = cred[0][tid];
+#pragma unroll
+                for (int r = 1; r < 16; ++r) t += cred[r][tid];
+                sums[tm * K + k0 + tid] = t;
+            }
     }
 }
 
@@ -618,24 +671,32 @@ int fp8_launch(K kernel, const Fp8Plan& p, int threads, int smem, const Fp8Args&
 
 extern "C" int64_t sgg_fp8_scale_bytes(int64_t rows, int64_t K) { return rows < 0 || K < 0 ? SGG_ERR_ARG : scale_bytes(rows, (K + 127) / 128); }
 
-extern "C" int sgg_fp8_quantize(const void* x, int64_t ldx, int64_t M, int64_t K, void* rows, void* rows_scale, void* cols, void* cols_scale, int dtype,
-                                void* stream) {
+extern "C" int sgg_fp8_quantize(const void* x, int64_t ldx, int64_t M, int64_t K, void* rows, void* rows_scale, void* cols, void* cols_scale, float* colsum,
+                                float* colsum_ws, int dtype, void* stream) {
     if (!sgg_is_dtype(dtype)) return SGG_ERR_DTYPE;
-    if (M < 0 || K < 0 || M > 0x7fffff00 || K > 0x7fffff00 || ldx < K || (!rows && !cols) || !rows != !rows_scale || !cols != !cols_scale) return SGG_ERR_ARG;
-    if (((uintptr_t)rows | (uintptr_t)cols) & 15) return SGG_ERR_ARG;
-    if (M == 0 || K == 0) return SGG_OK;
-    if (!x) return SGG_ERR_ARG;
+    if (M < 0 || K < 0 || M > 0x7fffff00 || K > 0x7fffff00 || ldx < K || (colsum && !colsum_ws)) return SGG_ERR_ARG;
+    if (M > 0 && K > 0 && ((!rows && !cols) || !rows != !rows_scale || !cols != !cols_scale || (colsum && !cols))) return SGG_ERR_ARG;       // (empty forms have no memory)
+    if ((((uintptr_t)rows | (uintptr_t)cols) & 15) || (((uintptr_t)rows_scale | (uintptr_t)cols_scale) & 3)) return SGG_ERR_ARG;
     const int64_t tilesM = (M + 127) / 128, tilesK = (K + 127) / 128;
     if (tilesM * tilesK > 0x7fffffff) return SGG_ERR_ARG;
+    if (M > 0 && K > 0 && !x) return SGG_ERR_ARG;
     hipStream_t s = (hipStream_t)stream;
-#define SGG_Q(R_, C_)                                                                                                                               \
-    SGG_FOR_DTYPE(dtype, hipLaunchKernelGGL((fp8_quantize_kernel<T, R_, C_>), dim3((unsigned)(tilesM * tilesK)), dim3(256), 0, s, (const T*)x, (long)ldx, \
-                                            (long)M, (int)K, (unsigned char*)rows, (unsigned char*)rows_scale, (unsigned char*)cols,                 \
-                                            (unsigned char*)cols_scale, (int)tilesM))
-    if (rows && cols) { SGG_Q(true, true); } else if (rows) { SGG_Q(true, false); } else { SGG_Q(false, true); }
+    if (M > 0 && K > 0) {
+#define SGG_Q(R_, C_, S_)                                                                                                                               \
+    SGG_FOR_DTYPE(dtype, hipLaunchKernelGGL((fp8_quantize_kernel<T, R_, C_, S_>), dim3((unsigned)(tilesM * tilesK)), dim3(256), 0, s, (const T*)x, (long)ldx, \
+                                            (long)M, (int)K, (unsigned char*)rows, (unsigned char*)rows_scale, (unsigned char*)cols,                       \
+                                            (unsigned char*)cols_scale, colsum_ws, (int)tilesK))
+        if (rows && cols) {
+            if (colsum) { SGG_Q(true, true, true); } else { SGG_Q(true, true, false); }
+        } else if (cols) {
+            if (colsum) { SGG_Q(false, true, true); } else { SGG_Q(false, true, false); }
+        } else {
+            SGG_Q(true, false, false);
+        }
 #undef SGG_Q
-    SGG_CHECK_LAUNCH();
-    return SGG_OK;
+        SGG_CHECK_LAUNCH();
+    }
+    return colsum && K > 0 ? sgg_reduce_parts(colsum_ws, (int)tilesM, (int)K, colsum, 0, s) : SGG_OK;
 }
 
 // K slices of a product whose output tiles alone do not fill the chip; ws then holds that many fp32 [M][N] partial outputs

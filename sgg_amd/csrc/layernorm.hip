@@ -81,6 +81,22 @@ struct LnShape {
     static constexpr int CAP = LPR * WPR * NV * 8;                                  // columns
 };
 
+// the lane's columns of a per-column vector (fill where there is none)
+template <typename L, int NV>
+__device__ __forceinline__ void load_columns(const float* p, const L& at, float fill, float (&v)[NV][8]) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if (p && at.n[i] > 0) {
+            Piece<float> q;
+            q.load(p + at.col[i], at.n[i]);
+            q.get(v[i]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = fill;
+        }
+    }
+}
+
 // sum over the lanes of a row; every lane of the row gets it.  red: WAVES floats of LDS, a set of its own per call inside one row (no lane can be two
 // calls ahead of another: the barriers in between)
 template <typename S>
@@ -122,13 +138,8 @@ __global__ __launch_bounds__(S::THREADS) void ln_fwd_kernel(const T* __restrict_
     __shared__ float red[2][S::WAVES];
     const LnLane<S> at(C);
     float wv[S::NV][8], bv[S::NV][8];
-#pragma unroll
-    for (int i = 0; i < S::NV; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            wv[i][j] = w && j < at.n[i] ? w[at.col[i] + j] : 1.f;
-            bv[i][j] = b && j < at.n[i] ? b[at.col[i] + j] : 0.f;
-        }
+    load_columns(w, at, 1.f, wv);
+    load_columns(b, at, 0.f, bv);
     const long step = (long)gridDim.x * S::GROUPS;
     const float invC = 1.f / (float)C;
     Piece<T> p[S::NV];
@@ -194,14 +205,8 @@ __global__ __launch_bounds__(S::THREADS) void ln_bwd_kernel(const T* __restrict_
     __shared__ float red[2][S::WAVES];
     __shared__ float fold[DW && S::GROUPS > 1 ? S::GROUPS * S::CAP : 1];
     const LnLane<S> at(C);
-    float wv[S::NV][8], aw[S::NV][8], ab[S::NV][8];
-#pragma unroll
-    for (int i = 0; i < S::NV; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            wv[i][j] = w && j < at.n[i] ? w[at.col[i] + j] : 1.f;
-            aw[i][j] = ab[i][j] = 0.f;
-        }
+    float wv[S::NV][8], aw[S::NV][8] = {}, ab[S::NV][8] = {};
+    load_columns(w, at, 1.f, wv);
     const long step = (long)gridDim.x * S::GROUPS;
     const float invC = 1.f / (float)C;
     Piece<T> px[S::NV], pg[S::NV];

@@ -155,18 +155,21 @@ class _AffineFp8(torch.autograd.Function):
         need_dx, need_dw = need_dx and wt is not None, need_dw and xt is not None
         dy = _row_form(dy)
         dq = dt = dx = dw = db = None
-        if need_dx and need_dw:
-            dq, dt = ops.quantize_fp8(dy, 'both')
-        elif need_dx:
-            dq = ops.quantize_fp8(dy)
-        elif need_dw:
-            dt = ops.quantize_fp8(dy, 'cols')
+        if need_dw:                                  # the bias gradient rides along: column sums out of the same reading of dy
+            q = ops.quantize_fp8(dy, 'both' if need_dx else 'cols', colsum=need_db)
+            q, db = q if need_db else (q, None)
+            dq, dt = q if need_dx else (None, q)
+        else:
+            if need_dx:
+                dq = ops.quantize_fp8(dy)
+            if need_db:
+                db = ops.colsum(dy.contiguous()) if dy.shape[0] else dy.new_zeros(dy.shape[1], dtype=torch.float32)
         if need_dx:
             dx = ops.gemm_fp8(dq, wt, out_dtype=ctx.types[0])
         if need_dw:
             dw = ops.gemm_fp8(dt, xt).to(ctx.types[1])
-        if need_db:
-            db = (ops.colsum(dy.contiguous()) if dy.shape[0] else dy.new_zeros(dy.shape[1], dtype=torch.float32)).to(ctx.types[2])
+        if db is not None:
+            db = db.to(ctx.types[2])
         return dx, dw, db, None
 
 
@@ -315,19 +318,17 @@ class BatchNormRows(nn.modules.batchnorm._BatchNorm):
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, eps):
-        xr = _row_form(x)
-        need = any(ctx.needs_input_grad[:3])
-        y, mean, rstd = ops.layer_norm(xr, w, b, eps, stats=need)
-        if need:
-            ctx.save_for_backward(xr, mean, rstd, *([w] if w is not None else []))
+        x = _row_form(x)
+        y, stats = ops._layer_norm(x, w, b, eps, True)
+        ctx.save_for_backward(x, stats, w)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        xr, mean, rstd = ctx.saved_tensors[:3]
-        w = ctx.saved_tensors[3] if len(ctx.saved_tensors) > 3 else None
-        return ops.layer_norm_bwd(_row_form(dy), xr, mean, rstd, w, *ctx.needs_input_grad[:3]) + (None,)
+        x, stats, w = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        return ops.layer_norm_bwd(_row_form(dy), x, stats[0], stats[1], w, need[0], need[1], need[2]) + (None,)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
@@ -335,8 +336,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     -> x's shape and type; differentiable in all three (csrc/layernorm.hip: one pass each way)."""
     _need_gpu(x)
     rows = x.reshape(-1, x.shape[-1])
-    if not torch.is_grad_enabled():
-        return ops.layer_norm(_row_form(rows), weight, bias, eps, stats=False)[0].view(x.shape)
+    if not (torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad))):
+        return ops._layer_norm(_row_form(rows), weight, bias, eps, False)[0].view(x.shape)
     return _LayerNorm.apply(rows, weight, bias, eps).view(x.shape)
 
 

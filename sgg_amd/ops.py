@@ -1205,19 +1205,25 @@ def _vector(t, n, what):
     return _p(t, torch.float32)
 
 
-def layer_norm(x, weight=None, bias=None, eps=1e-5, stats=True):
-    """x [M, C] (f32 / bf16 / f16, row-strided ok) -> (y [M, C] in x's type, mean f32[M], rstd f32[M]); weight, bias f32[C] or None.
-    stats=False: (y, None, None)."""
+def _layer_norm(x, weight, bias, eps, stats):
+    """-> (y, f32[2, M] = means and reciprocal deviations, or None)"""
     _here(x, 'layer_norm')
     ld, (M, C) = _row_matrix(x, 'layer_norm'), x.shape
     if not 1 <= C <= LAYER_NORM_MAX:
         raise ValueError('sgg_amd: layer_norm: rows of 1 .. %d columns, got %d' % (LAYER_NORM_MAX, C))
     w, b = _vector(weight, C, 'layer_norm weight'), _vector(bias, C, 'layer_norm bias')
     y = torch.empty((M, C), dtype=x.dtype, device=x.device)
-    mean, rstd = torch.empty((2, M), dtype=torch.float32, device=x.device) if stats else (None, None)
-    _lib.call('sgg_layer_norm_fwd', x.data_ptr(), ld, w, b, y.data_ptr(), mean.data_ptr() if stats else None, rstd.data_ptr() if stats else None,
-              M, C, float(eps), dt(x), _stream())
-    return y, mean, rstd
+    st = torch.empty((2, M), dtype=torch.float32, device=x.device) if stats else None
+    mean = st.data_ptr() if stats else None
+    _lib.call('sgg_layer_norm_fwd', x.data_ptr(), ld, w, b, y.data_ptr(), mean, mean + 4 * M if mean else mean, M, C, eps, dt(x), _stream())
+    return y, st
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, stats=True):
+    """x [M, C] (f32 / bf16 / f16, row-strided ok) -> (y [M, C] in x's type, mean f32[M], rstd f32[M]); weight, bias f32[C] or None.
+    stats=False: (y, None, None)."""
+    y, st = _layer_norm(x, weight, bias, eps, stats)
+    return (y, st[0], st[1]) if stats else (y, None, None)
 
 
 def layer_norm_bwd(dy, x, mean, rstd, weight=None, want_dx=True, want_dw=True, want_db=True):
@@ -1271,20 +1277,26 @@ def _fp8_empty(M, K, device):
                    torch.empty(_lib.load().sgg_fp8_scale_bytes(M, K), dtype=torch.uint8, device=device), (M, K))
 
 
-def quantize_fp8(x, form='rows'):
+def quantize_fp8(x, form='rows', colsum=False):
     """x [M, K] (f32 / bf16 / f16, row-strided ok) -> its 8-bit operand form: form 'rows' Fp8Rows of x, 'cols' Fp8Rows of x^T (blocks of 128
-    rows of x share a scale), 'both' the pair of them out of one reading of x.  Non-finite elements become NaN."""
+    rows of x share a scale), 'both' the pair of them out of one reading of x.  Non-finite elements become NaN.
+    colsum=True ('cols' / 'both'): -> (what it gives otherwise, column sums of x f32[K]) -- the bias gradient of x = dY, out of the same reading."""
     if form not in ('rows', 'cols', 'both'):
         raise ValueError("sgg_amd: quantize_fp8: form must be 'rows', 'cols' or 'both', got %r" % (form,))
+    if colsum and form == 'rows':
+        raise ValueError("sgg_amd: quantize_fp8: column sums come with the forms 'cols' and 'both'")
     _here(x, 'quantize_fp8')
     ld, (M, K) = _row_matrix(x, 'quantize_fp8'), x.shape
     code = dt(x)
     r = _fp8_empty(M, K, x.device) if form != 'cols' else None
     c = _fp8_empty(K, M, x.device) if form != 'rows' else None
-    if M and K:
-        _lib.call('sgg_fp8_quantize', x.data_ptr(), ld, M, K, r.data.data_ptr() if r else None, r.scale.data_ptr() if r else None,
-                  c.data.data_ptr() if c else None, c.scale.data_ptr() if c else None, code, _stream())
-    return r if c is None else c if r is None else (r, c)
+    sums = torch.empty(K, dtype=torch.float32, device=x.device) if colsum else None
+    ws = _ws((M + 127) // 128 * K, x.device) if colsum else None
+    _lib.call('sgg_fp8_quantize', x.data_ptr(), ld, M, K, r.data.data_ptr() if r else None, r.scale.data_ptr() if r else None,
+              c.data.data_ptr() if c else None, c.scale.data_ptr() if c else None, sums.data_ptr() if colsum else None, ws.data_ptr() if colsum else None,
+              code, _stream())
+    out = r if c is None else c if r is None else (r, c)
+    return (out, sums) if colsum else out
 
 
 def gemm_fp8(A, W, bias=None, act=ACT_NONE, out_dtype=torch.float32, out=None):

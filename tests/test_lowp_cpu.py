@@ -36,10 +36,11 @@ def test_fp8_entries_refuse():
     from sgg_amd import _lib
     lib = _lib.load()
 
-    def q(x=P, ldx=256, M=4, K=256, rows=P, rs=P, cols=P, cs=P, dtype=0):
-        return lib.sgg_fp8_quantize(x, ldx, M, K, rows, rs, cols, cs, dtype, None)
+    def q(x=P, ldx=256, M=4, K=256, rows=P, rs=P, cols=P, cs=P, sums=None, ws=None, dtype=0):
+        return lib.sgg_fp8_quantize(x, ldx, M, K, rows, rs, cols, cs, sums, ws, dtype, None)
     for bad in (dict(x=None), dict(ldx=255), dict(M=-1), dict(K=-1), dict(rows=None), dict(rs=None), dict(cols=None), dict(cs=None),
-                dict(rows=None, rs=None, cols=None, cs=None), dict(rows=P + 8), dict(cols=P + 4), dict(M=1 << 40)):
+                dict(rows=None, rs=None, cols=None, cs=None), dict(rows=P + 8), dict(cols=P + 4), dict(rs=P + 2), dict(M=1 << 40),
+                dict(sums=P), dict(sums=P, ws=P, cols=None, cs=None)):
         assert q(**bad) == ERR_ARG, bad
     assert q(dtype=5) == ERR_DTYPE and q(M=0, x=None) == 0
 
