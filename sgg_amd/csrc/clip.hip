@@ -7,7 +7,7 @@ namespace {
 
 constexpr int CLIP_TAB = 96;            // tensors per launch (the table travels by value in the kernel arguments)
 constexpr int CLIP_CHUNK = 8192;        // elements a workgroup takes at a time
-constexpr int CLIP_BLOCKS = 1024;       // partials per launch: 4 workgroups per CU
+constexpr int CLIP_BLOCKS = 2048;       // partials per launch: 8 workgroups per CU
 constexpr int CLIP_SMALL = 8;           // chunks up to which one workgroup does it all
 
 struct ClipTab {

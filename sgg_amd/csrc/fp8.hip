@@ -260,12 +260,13 @@ __device__ __forceinline__ void out_row8(const Fp8Args& g, const float (&bias8)[
     }
 }
 
-// a wave's 32 MI x 64 outputs, from fragments whose lanes hold one row m and 4 consecutive n per register quad, to rows of 8 consecutive n per lane
+// a wave's 32 MI x 32 NI outputs, from fragments whose lanes hold one row m and 4 consecutive n per register quad, to rows of 8 consecutive n per lane
 // through 8.5 KiB of LDS of its own (est; row stride 272 bytes)
 constexpr int EST = 32 * 272;
-template <int MI>
-__device__ __forceinline__ void out_wave(const Fp8Args& g, f32x16 (&acc)[MI][2], char* est, long m0, long n0, float* part) {
-    const int lane = threadIdx.x & 63, fr = lane & 31, fh = lane >> 5, rl = lane >> 3, cl = (lane & 7) * 8;
+template <int MI, int NI>
+__device__ __forceinline__ void out_wave(const Fp8Args& g, f32x16 (&acc)[MI][NI], char* est, long m0, long n0, float* part) {
+    constexpr int LN = 4 * NI, ROWS = 64 / LN;                // lanes along a row, rows at a time
+    const int lane = threadIdx.x & 63, fr = lane & 31, fh = lane >> 5, rl = lane / LN, cl = (lane % LN) * 8;
     const long n = n0 + cl;
     const int nv = (int)min(8L, max(0L, (long)g.N - n));
     float bias8[8];
@@ -274,17 +275,17 @@ __device__ __forceinline__ void out_wave(const Fp8Args& g, f32x16 (&acc)[MI][2],
 #pragma unroll
     for (int mi = 0; mi < MI; ++mi) {
 #pragma unroll
-        for (int ni = 0; ni < 2; ++ni)
+        for (int ni = 0; ni < NI; ++ni)
 #pragma unroll
             for (int c = 0; c < 4; ++c)
                 *reinterpret_cast<f32x4*>(est + fr * 272 + (ni * 32 + 8 * c + 4 * fh) * 4) =
                     f32x4{acc[mi][ni][4 * c], acc[mi][ni][4 * c + 1], acc[mi][ni][4 * c + 2], acc[mi][ni][4 * c + 3]};
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                               // (its own writes: no other wave reads them)
 #pragma unroll
-        for (int it = 0; it < 4; ++it) {
-            const long m = m0 + mi * 32 + rl + 8 * it;
-            const f32x4 lo = *reinterpret_cast<const f32x4*>(est + (rl + 8 * it) * 272 + cl * 4);
-            const f32x4 hi = *reinterpret_cast<const f32x4*>(est + (rl + 8 * it) * 272 + cl * 4 + 16);
+        for (int it = 0; it < 32 / ROWS; ++it) {
+            const long m = m0 + mi * 32 + rl + ROWS * it;
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(est + (rl + ROWS * it) * 272 + cl * 4);
+            const f32x4 hi = *reinterpret_cast<const f32x4*>(est + (rl + ROWS * it) * 272 + cl * 4 + 16);
             float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
             if (m < g.M && nv > 0) out_row8(g, bias8, v, m, n, nv, part);
         }
@@ -318,16 +319,25 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(const Fp8Args g, const fl
     }
 }
 
+// Workgroup -> (tile, K slice).  One-dimensional grid of tiles x slices; consecutive logical ids run on one XCD (its own L2): a slice's tiles together, so that
+// the slice's columns of A are fetched into one L2 once and not into all eight.
+__device__ __forceinline__ void tile_and_slice(int tilesM, int tilesN, int& tm, int& tn, int& slice) {
+    const int tiles = tilesM * tilesN, logical = xcd_remap(blockIdx.x, gridDim.x);
+    slice = logical / tiles;
+    tile_coords_logical(logical - slice * tiles, tilesM, tilesN, tm, tn);
+}
+
 // ---- (1) up to 32 rows of A: a stream of W.  Bound by reading W once (its bytes / the memory's rate); everything else hides behind that.  A workgroup
 // owns 32 rows of W and a K slice, its 4 waves take the slice's blocks in turn (four neighbouring 128-byte pieces of every row are in flight together)
 // straight into registers, DEPTH blocks ahead of their use; the waves' sums meet in LDS.  Always the bf16 pipe: the conversions are a tenth of the
 // time W takes to arrive.
 template <int DEPTH>
-__global__ __launch_bounds__(256) void fp8_few_rows_kernel(const Fp8Args g, float* __restrict__ ws, int per) {
+__global__ __launch_bounds__(256) void fp8_few_rows_kernel(const Fp8Args g, float* __restrict__ ws, int per, int slices) {
     __shared__ float red[4][32 * 33];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 31, fh = lane >> 5;
-    const long n0 = (long)blockIdx.x * 32;
-    const int blocks = (int)(g.Kp / 128), b0 = min((int)blockIdx.y * per, blocks), b1 = min(b0 + per, blocks);
+    const int slice = blockIdx.x % slices;
+    const long n0 = (long)(blockIdx.x / slices) * 32;
+    const int blocks = (int)(g.Kp / 128), b0 = min(slice * per, blocks), b1 = min(b0 + per, blocks);
     const long gA = ((long)g.M + 127) / 128, gW = ((long)g.N + 127) / 128;
     const unsigned char* wp = g.W + min(n0 + fr, (long)g.N - 1) * g.Kp + fh * 16;
     const unsigned char* ap = g.A + (long)min(fr, g.M - 1) * g.Kp + fh * 16;
@@ -360,7 +370,7 @@ __global__ __launch_bounds__(256) void fp8_few_rows_kernel(const Fp8Args g, floa
 #pragma unroll
     for (int r = 0; r < 16; ++r) red[wave][fr * 33 + 8 * (r >> 2) + 4 * fh + (r & 3)] = acc[r];
     __syncthreads();
-    float* part = gridDim.y > 1 ? ws + (long)blockIdx.y * g.M * g.N : nullptr;
+    float* part = slices > 1 ? ws + (long)slice * g.M * g.N : nullptr;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int m = i * 8 + (tid >> 5);
@@ -377,17 +387,75 @@ __global__ __launch_bounds__(256) void fp8_few_rows_kernel(const Fp8Args g, floa
     }
 }
 
+// The same for up to 16 rows: 16 rows of W per workgroup and 16 waves over K, so that 4096 rows of W already occupy every CU without K slices whose
+// partial outputs a second launch would have to add.
+template <int DEPTH>
+__global__ __launch_bounds__(1024) void fp8_few16_kernel(const Fp8Args g, float* __restrict__ ws, int per, int slices) {
+    __shared__ float red[16][16 * 17];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, fq = lane >> 4;
+    const int slice = blockIdx.x % slices;
+    const long n0 = (long)(blockIdx.x / slices) * 16;
+    const int blocks = (int)(g.Kp / 128), b0 = min(slice * per, blocks), b1 = min(b0 + per, blocks);
+    const long gA = ((long)g.M + 127) / 128, gW = ((long)g.N + 127) / 128;
+    const long n = min(n0 + fr, (long)g.N - 1);
+    const unsigned char* wp = g.W + n * g.Kp + fq * 16;
+    const unsigned char* ap = g.A + (long)min(fr, g.M - 1) * g.Kp + fq * 16;
+    const unsigned* sw = reinterpret_cast<const unsigned*>(g.Ws) + (n >> 7) * 32 + (n & 31);
+    const unsigned* sa = reinterpret_cast<const unsigned*>(g.As) + fr;
+    const int shift = (int)(n >> 5 & 3) * 8;
+    struct { u32x4 w[2], a[2]; unsigned ew, ea; } buf[DEPTH];
+    auto fetch = [&](auto& t, int b) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            t.w[c] = *reinterpret_cast<const u32x4*>(wp + (long)b * 128 + c * 64);
+            t.a[c] = *reinterpret_cast<const u32x4*>(ap + (long)b * 128 + c * 64);
+        }
+        t.ew = sw[(long)b * gW * 32];
+        t.ea = sa[(long)b * gA * 32];
+    };
+    f32x4 acc = {};
+#pragma unroll
+    for (int u = 0; u < DEPTH; ++u)
+        if (b0 + wave + 16 * u < b1) fetch(buf[u], b0 + wave + 16 * u);
+    for (int b = b0 + wave; b < b1; b += 16 * DEPTH) {
+#pragma unroll
+        for (int u = 0; u < DEPTH; ++u) {
+            if (b + 16 * u >= b1) continue;
+            const Wide w = widen(join8(buf[u].w[0], buf[u].w[1]), scale_f32<0>(buf[u].ew >> shift)), a = widen(join8(buf[u].a[0], buf[u].a[1]), scale_f32<0>(buf[u].ea));
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, w.c[c]), __builtin_bit_cast(bf16x8_t, a.c[c]), acc, 0, 0, 0);
+            if (b + 16 * (u + DEPTH) < b1) fetch(buf[u], b + 16 * (u + DEPTH));
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) red[wave][fr * 17 + 4 * fq + r] = acc[r];                // row m = fr, columns n0 + 4 fq + r
+    __syncthreads();
+    const int m = tid >> 4;
+    const long no = n0 + (tid & 15);
+    if (m >= 16 || m >= g.M || no >= g.N) return;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) v += red[w][m * 17 + (tid & 15)];
+    if (slices > 1) {
+        ws[((long)slice * g.M + m) * g.N + no] = v;
+    } else {
+        v += g.bias ? g.bias[no] : 0.f;
+        out_st(g.C, m * g.ldc + no, g.out_dt, g.act == SGG_ACT_RELU && v < 0.f ? 0.f : v);
+    }
+}
+
 // ---- (2) the middle: tiles of 128 x 128, 4 waves of 64 x 64, one block of 128 per step, K slices while the tiles do not fill the chip.  Two LDS buffers
 // of 32 KiB (two workgroups per CU): while one block is multiplied, the next one's loads are in flight to registers.
 template <bool WIDE>
-__global__ __launch_bounds__(256) void fp8_tile_kernel(const Fp8Args g, float* __restrict__ ws, int per) {
+__global__ __launch_bounds__(256) void fp8_tile_kernel(const Fp8Args g, float* __restrict__ ws, int per, int slices) {
     __shared__ __attribute__((aligned(16))) unsigned char sm[2][2][128 * 128];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int tm, tn;
-    tile_coords(blockIdx.x, (g.M + 127) / 128, (g.N + 127) / 128, tm, tn);
+    int tm, tn, slice;
+    tile_and_slice((g.M + 127) / 128, (g.N + 127) / 128, tm, tn, slice);
     const long m0 = (long)tm * 128, n0 = (long)tn * 128;
     const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64, fr = lane & 31, fh = lane >> 5;
-    const int blocks = (int)(g.Kp / 128), b0 = min((int)blockIdx.y * per, blocks), b1 = min(b0 + per, blocks);
+    const int blocks = (int)(g.Kp / 128), b0 = min(slice * per, blocks), b1 = min(b0 + per, blocks);
     const long gA = ((long)g.M + 127) / 128, gW = ((long)g.N + 127) / 128;
     const unsigned *sa = reinterpret_cast<const unsigned*>(g.As) + (long)tm * 32 + fr, *sw = reinterpret_cast<const unsigned*>(g.Ws) + (long)tn * 32 + fr;
     // thread -> rows tid / 8 + 32 p, 16-byte piece tid % 8, stored at the piece permuted by the row (reads of 32 rows then spread over the banks)
@@ -450,16 +518,16 @@ __global__ __launch_bounds__(256) void fp8_tile_kernel(const Fp8Args g, float* _
         }
     }
     __syncthreads();                                          // (the staging below lies over the operand buffers)
-    out_wave<2>(g, acc, reinterpret_cast<char*>(sm) + wave * EST, m0 + wm, n0 + wn, gridDim.y > 1 ? ws + (long)blockIdx.y * g.M * g.N : nullptr);
+    out_wave<2, 2>(g, acc, reinterpret_cast<char*>(sm) + wave * EST, m0 + wm, n0 + wn, slices > 1 ? ws + (long)slice * g.M * g.N : nullptr);
 }
 
-// ---- (3) large: tiles of 256 x 256, 8 waves = two groups of four, one wave of each group per SIMD; a wave owns 128 x 64.  K advances in slabs of 64 bytes
-// per row (half a block).  The groups run the same slabs one phase apart, one barrier per phase: while one group's waves read their fragments of a slab
+// ---- (3) large: tiles of 256 x 128 NI, 8 waves = two groups of four, one wave of each group per SIMD; a wave owns 128 x 32 NI.  K advances in slabs of 64
+// bytes per row (half a block).  The groups run the same slabs one phase apart, one barrier per phase: while one group's waves read their fragments of a slab
 // from LDS (and, for fp32 outputs, widen them), the other group's waves hold the matrix pipe:
 //   slot      0        1        2        3        4   ...
 //   group 0   LOAD 0   MFMA 0   LOAD 1   MFMA 1   LOAD 2
 //   group 1   -        LOAD 0   MFMA 0   LOAD 1   MFMA 1
-// A ring of 4 slabs (4 x 32 KiB) is filled by loads straight to LDS, three slabs ahead, issued between the matrix instructions and counted (never
+// A ring of D = 4 slabs (NI = 2: 4 x 32 KiB) is filled by loads straight to LDS, D - 1 slabs ahead, issued between the matrix instructions and counted (never
 // drained before the end).  With a block's first slab travels the wave's own 256 bytes of scales: 32 dwords of its 128 rows of A, 32 of its rows of W.
 // 16-byte pieces of a row are permuted by (row / 4) % 4 on the source address and on the read: fragment reads of 32 rows hit every bank once.
 // one piece: uniform base + lane offset + immediate.  (The empty asm keeps the offset's widening next to the load, where it folds into the instruction's
@@ -471,87 +539,103 @@ __device__ __forceinline__ void lds_piece(const char* ubase, unsigned& off, char
     __builtin_amdgcn_global_load_lds((glb_void_t*)(ubase + off), (lds_void_t*)l, 16, OFF, 0);
 }
 
-constexpr int PP_ROW = 64, PP_STAGE = 512 * PP_ROW, PP_RING = 4 * PP_STAGE, PP_SMEM = PP_RING + 4 * 8 * 256;
+constexpr int PP_ROW = 64;
+constexpr int pp_stage(int NI) { return (256 + 128 * NI) * PP_ROW; }
+constexpr int PP_DEPTH = 4;                                           // slabs of the ring (even; 6 measured no faster)
+constexpr int pp_smem(int NI) { return PP_DEPTH * pp_stage(NI) + 4 * 8 * 256; }
 
-template <bool WIDE>
-__global__ __launch_bounds__(512) void fp8_pingpong_kernel(const Fp8Args g, float* __restrict__ ws, int per) {
+template <bool WIDE, int NI>
+__global__ __launch_bounds__(512) void fp8_pingpong_kernel(const Fp8Args g, float* __restrict__ ws, int per, int slices) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
+    constexpr int D = PP_DEPTH, PP_STAGE = pp_stage(NI), PP_RING = D * PP_STAGE, PIECES = 2 + NI;
+    static_assert(8 * EST <= PP_RING, "the output staging lies over the ring");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int grp = wave >> 2, q = wave & 3, fr = lane & 31, fh = lane >> 5;
-    int tm, tn;
-    tile_coords(blockIdx.x, (g.M + 255) / 256, (g.N + 255) / 256, tm, tn);
-    const long m0 = (long)tm * 256, n0 = (long)tn * 256;
-    const int blocks = (int)(g.Kp / 128), b0 = min((int)blockIdx.y * per, blocks), b1 = min(b0 + per, blocks);
+    int tm, tn, slice;
+    tile_and_slice((g.M + 255) / 256, (g.N + 128 * NI - 1) / (128 * NI), tm, tn, slice);
+    const long m0 = (long)tm * 256, n0 = (long)tn * 128 * NI;
+    const int blocks = (int)(g.Kp / 128), b0 = min(slice * per, blocks), b1 = min(b0 + per, blocks);
     const int kb = 2 * b0, nt = 2 * b1;                       // slabs of this slice
 
-    // ---- loads to LDS: waves 0-3 the rows of A, waves 4-7 those of W; 4 instructions of 16 rows.  Global address = uniform base + a lane offset that
-    // never changes + the instruction's immediate, which also moves the LDS address: piece j lands j KiB behind ONE base (the lane offset carries
-    // -j KiB, and 3 KiB that the uniform base gives back keep it unsigned)
-    const bool loads_a = wave < 4;
-    const char* base = reinterpret_cast<const char*>(loads_a ? g.A + m0 * g.Kp : g.W + n0 * g.Kp);
-    unsigned vo[4];
+    // ---- loads to LDS: a slab is (16 + 8 NI) pieces of 16 rows, the rows of A, then those of W; wave w loads pieces PIECES w + j.  Global address = the
+    // piece's uniform base + a lane offset that never changes + the instruction's immediate, which also moves the LDS address: piece j lands j KiB
+    // behind ONE LDS base (the lane offset carries -j KiB, and 3 KiB that the uniform base gives back keep it unsigned)
+    const char *base_a = reinterpret_cast<const char*>(g.A + m0 * g.Kp) - 3072, *base_w = reinterpret_cast<const char*>(g.W + n0 * g.Kp) - 3072;
+    unsigned vo[4] = {};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int r = (wave & 3) * 64 + j * 16 + (lane >> 2);
-        const long row = loads_a ? min(m0 + r, (long)g.M - 1) - m0 : min(n0 + r, (long)g.N - 1) - n0;        // (rows past the end: the last one again)
+    for (int j = 0; j < PIECES; ++j) {
+        const int r = (PIECES * wave + j) * 16 + (lane >> 2);
+        const long row = r < 256 ? min(m0 + r, (long)g.M - 1) - m0 : min(n0 + r - 256, (long)g.N - 1) - n0;        // (rows past the end: the last one again)
         vo[j] = (unsigned)(row * g.Kp) + ((lane & 3) ^ ((r >> 2) & 3)) * 16 + 3072u - 1024u * j;
     }
     unsigned vo_0 = vo[0], vo_1 = vo[1], vo_2 = vo[2], vo_3 = vo[3];
-    const int lds_rows0 = (loads_a ? 0 : 256 * PP_ROW) + (wave & 3) * 64 * PP_ROW;
+    const char *const base_0 = PIECES * wave < 16 ? base_a : base_w, *const base_1 = PIECES * wave + 1 < 16 ? base_a : base_w,
+               *const base_2 = PIECES * wave + 2 < 16 ? base_a : base_w, *const base_3 = PIECES * wave + 3 < 16 ? base_a : base_w;
+    const int lds_rows0 = PIECES * wave * 16 * PP_ROW;
     const long gA = ((long)g.M + 127) / 128, gW = ((long)g.N + 127) / 128;
     const unsigned* sp = lane < 32 ? reinterpret_cast<const unsigned*>(g.As) + ((long)b0 * gA + min((long)tm * 2 + grp, gA - 1)) * 32 + fr
-                                   : reinterpret_cast<const unsigned*>(g.Ws) + ((long)b0 * gW + min((long)tn * 2 + (q >> 1), gW - 1)) * 32 + fr;
+                                   : reinterpret_cast<const unsigned*>(g.Ws) + ((long)b0 * gW + min(n0 / 128 + q * NI / 4, gW - 1)) * 32 + fr;
     const long sstep = (lane < 32 ? gA : gW) * 32;
     char* const sreg = smem + PP_RING + wave * 256;
     int sblock = b0;
-    // slabs are requested in order: kb .. nt - 1, then the last one three times more (into slabs of the ring that nobody reads again: the loop needs no tail)
+    // slabs are requested in order: kb .. nt - 1, then the last one D - 1 times more (into slabs of the ring that nobody reads again: the loop needs no tail)
     auto issue_scales = [&](int kt) {                         // with each even slab
         __builtin_amdgcn_global_load_lds((glb_void_t*)sp, (lds_void_t*)(sreg + ((kt >> 1) & 3) * 2048), 4, 0, 0);
         if (++sblock < b1) sp += sstep;
     };
-    auto slab_base = [&](int kt) { return uniform_ptr(base + (long)min(kt, nt - 1) * PP_ROW - 3072); };
+    auto slab_off = [&](int kt) { return (long)min(kt, nt - 1) * PP_ROW; };
     auto issue = [&](int kt) {
-        const char* ub = slab_base(kt);
-        char* dst = smem + (kt & 3) * PP_STAGE + lds_rows0;
+        const long k = slab_off(kt);
+        char* dst = smem + (kt % D) * PP_STAGE + lds_rows0;
         if (!(kt & 1)) issue_scales(kt);
-        lds_piece<0>(ub, vo_0, dst);
-        lds_piece<1024>(ub, vo_1, dst);
-        lds_piece<2048>(ub, vo_2, dst);
-        lds_piece<3072>(ub, vo_3, dst);
+        lds_piece<0>(uniform_ptr(base_0 + k), vo_0, dst);
+        lds_piece<1024>(uniform_ptr(base_1 + k), vo_1, dst);
+        lds_piece<2048>(uniform_ptr(base_2 + k), vo_2, dst);
+        if constexpr (NI == 2) lds_piece<3072>(uniform_ptr(base_3 + k), vo_3, dst);
     };
 
     // LDS byte addresses of the lane's pieces fh and fh + 2 in slab 0: its first row of A and of W (the others 32 rows = 2 KiB further, same permutation)
     const unsigned lds0 = (unsigned)(unsigned long)(lds_void_t*)smem;
-    const unsigned row_a = grp * 128 + fr, row_w = 256 + q * 64 + fr;
+    const unsigned row_a = grp * 128 + fr, row_w = 256 + q * 32 * NI + fr;
     const unsigned at_a = lds0 + row_a * PP_ROW + ((fh ^ ((row_a >> 2) & 3)) << 4), at_w = lds0 + row_w * PP_ROW + ((fh ^ ((row_w >> 2) & 3)) << 4);
     const unsigned at_s = lds0 + PP_RING + wave * 256 + fr * 4;
-    f32x16 acc[4][2] = {};
-    i32x8 af[4], wf[2];
-    Wide aw[4], ww[2];
+    f32x16 acc[4][NI] = {};
+    i32x8 af[4], wf[NI];
+    Wide aw[4], ww[NI];
     unsigned ea = 0, ew = 0;
     auto load_frags = [&](int kt, bool even) {
         // one asm block, with its wait: the compiler waits for EVERY load to LDS in flight before an LDS read of its own
-        const unsigned st = (kt & 3) * PP_STAGE;
+        const unsigned st = (kt % D) * PP_STAGE;
         const unsigned a0 = at_a + st, a1 = a0 ^ 32, w0 = at_w + st, w1 = w0 ^ 32;
         u32x4 f[12];
-#define FP8_READS                                                                                                              \
-    "ds_read_b128 %0, %14\n ds_read_b128 %1, %15\n ds_read_b128 %2, %14 offset:2048\n ds_read_b128 %3, %15 offset:2048\n"      \
-    "ds_read_b128 %4, %12\n ds_read_b128 %5, %13\n ds_read_b128 %6, %12 offset:2048\n ds_read_b128 %7, %13 offset:2048\n"      \
-    "ds_read_b128 %8, %12 offset:4096\n ds_read_b128 %9, %13 offset:4096\n ds_read_b128 %10, %12 offset:6144\n ds_read_b128 %11, %13 offset:6144\n"
-        asm volatile(FP8_READS "s_waitcnt lgkmcnt(0)"
-                     : "=&v"(f[0]), "=&v"(f[1]), "=&v"(f[2]), "=&v"(f[3]), "=&v"(f[4]), "=&v"(f[5]), "=&v"(f[6]), "=&v"(f[7]), "=&v"(f[8]), "=&v"(f[9]), "=&v"(f[10]), "=&v"(f[11])
-                     : "v"(a0), "v"(a1), "v"(w0), "v"(w1)
-                     : "memory");
-#undef FP8_READS
+        // outputs 0 .. 7 the fragments of A, 8 .. 11 those of W; inputs: A's two addresses, W's two
+#define FP8_READS_A(a0, a1)                                                                                                                    \
+    "ds_read_b128 %0, " a0 "\n ds_read_b128 %1, " a1 "\n ds_read_b128 %2, " a0 " offset:2048\n ds_read_b128 %3, " a1 " offset:2048\n"         \
+    "ds_read_b128 %4, " a0 " offset:4096\n ds_read_b128 %5, " a1 " offset:4096\n ds_read_b128 %6, " a0 " offset:6144\n ds_read_b128 %7, " a1 " offset:6144\n"
+        if constexpr (NI == 2) {
+            asm volatile("ds_read_b128 %8, %14\n ds_read_b128 %9, %15\n ds_read_b128 %10, %14 offset:2048\n ds_read_b128 %11, %15 offset:2048\n" FP8_READS_A("%12", "%13") "s_waitcnt lgkmcnt(0)"
+                         : "=&v"(f[0]), "=&v"(f[1]), "=&v"(f[2]), "=&v"(f[3]), "=&v"(f[4]), "=&v"(f[5]), "=&v"(f[6]), "=&v"(f[7]), "=&v"(f[8]), "=&v"(f[9]), "=&v"(f[10]), "=&v"(f[11])
+                         : "v"(a0), "v"(a1), "v"(w0), "v"(w1)
+                         : "memory");
+        } else {
+            asm volatile("ds_read_b128 %8, %12\n ds_read_b128 %9, %13\n" FP8_READS_A("%10", "%11") "s_waitcnt lgkmcnt(0)"
+                         : "=&v"(f[0]), "=&v"(f[1]), "=&v"(f[2]), "=&v"(f[3]), "=&v"(f[4]), "=&v"(f[5]), "=&v"(f[6]), "=&v"(f[7]), "=&v"(f[8]), "=&v"(f[9])
+                         : "v"(a0), "v"(a1), "v"(w0), "v"(w1)
+                         : "memory");
+        }
+#undef FP8_READS_A
         if (even) {
             unsigned e;
             asm volatile("ds_read_b32 %0, %2\n ds_read_b32 %1, %2 offset:128\n s_waitcnt lgkmcnt(0)" : "=&v"(ea), "=&v"(e) : "v"(at_s + ((kt >> 1) & 3) * 2048) : "memory");
-            ew = e >> ((q & 1) * 16);
+            ew = e >> (q * NI * 8 & 31);                       // bytes: the wave's NI rows-of-32 inside the group of 128
         }
-        wf[0] = join8(f[0], f[1]); wf[1] = join8(f[2], f[3]);
-        af[0] = join8(f[4], f[5]); af[1] = join8(f[6], f[7]); af[2] = join8(f[8], f[9]); af[3] = join8(f[10], f[11]);
+        wf[0] = join8(f[8], f[9]);
+        if constexpr (NI == 2) wf[NI - 1] = join8(f[10], f[11]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) af[i] = join8(f[2 * i], f[2 * i + 1]);
         if constexpr (WIDE) {
-            ww[0] = widen(wf[0], scale_f32<0>(ew)); ww[1] = widen(wf[1], scale_f32<1>(ew));
+            ww[0] = widen(wf[0], scale_f32<0>(ew));
+            if constexpr (NI == 2) ww[NI - 1] = widen(wf[NI - 1], scale_f32<1>(ew));
             aw[0] = widen(af[0], scale_f32<0>(ea)); aw[1] = widen(af[1], scale_f32<1>(ea));
             aw[2] = widen(af[2], scale_f32<2>(ea)); aw[3] = widen(af[3], scale_f32<3>(ea));
         }
@@ -560,28 +644,29 @@ __global__ __launch_bounds__(512) void fp8_pingpong_kernel(const Fp8Args g, floa
 #define FP8_MMA(mi)                                                                                                                              \
     if constexpr (WIDE) {                                                                                                                        \
         mma_wide(acc[mi][0], ww[0], aw[mi]);                                                                                                     \
-        mma_wide(acc[mi][1], ww[1], aw[mi]);                                                                                                     \
+        if constexpr (NI == 2) mma_wide(acc[mi][NI - 1], ww[NI - 1], aw[mi]);                                                                    \
     } else {                                                                                                                                     \
         acc[mi][0] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[0], af[mi], acc[mi][0], 0, 0, 0, ew, mi, ea);                             \
-        acc[mi][1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[1], af[mi], acc[mi][1], 0, 0, 1, ew, mi, ea);                             \
+        if constexpr (NI == 2) acc[mi][NI - 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[NI - 1], af[mi], acc[mi][NI - 1], 0, 0, 1, ew, mi, ea); \
     }
     auto compute_dma = [&](int pf, bool scales) {             // the slab's matrix instructions with the loads of slab pf between them
-        const char* ub = slab_base(pf);
-        char* dst = smem + (pf & 3) * PP_STAGE + lds_rows0;
+        const long k = slab_off(pf);
+        const char *u0 = uniform_ptr(base_0 + k), *u1 = uniform_ptr(base_1 + k), *u2 = uniform_ptr(base_2 + k), *u3 = uniform_ptr(base_3 + k);
+        char* dst = smem + (pf % D) * PP_STAGE + lds_rows0;
         if (scales) issue_scales(pf);
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_setprio(1);
         FP8_MMA(0)
-        lds_piece<0>(ub, vo_0, dst);
+        lds_piece<0>(u0, vo_0, dst);
         __builtin_amdgcn_sched_barrier(0);
         FP8_MMA(1)
-        lds_piece<1024>(ub, vo_1, dst);
+        lds_piece<1024>(u1, vo_1, dst);
         __builtin_amdgcn_sched_barrier(0);
         FP8_MMA(2)
-        lds_piece<2048>(ub, vo_2, dst);
+        lds_piece<2048>(u2, vo_2, dst);
         __builtin_amdgcn_sched_barrier(0);
         FP8_MMA(3)
-        lds_piece<3072>(ub, vo_3, dst);
+        if constexpr (NI == 2) lds_piece<3072>(u3, vo_3, dst);
         __builtin_amdgcn_s_setprio(0);
         __builtin_amdgcn_sched_barrier(0);
     };
@@ -592,26 +677,26 @@ __global__ __launch_bounds__(512) void fp8_pingpong_kernel(const Fp8Args g, floa
         asm volatile("" ::: "memory");    \
         __builtin_amdgcn_sched_barrier(0);\
     }
-    // Waits.  A wave issues 5 loads with an even slab (scales first), 4 with an odd one, slabs in order.  Before the barrier behind which slab kt + 1 is
-    // read, a wave may still have in flight what it issued after slab kt + 1: group 0 (at the end of MFMA kt, having issued kt + 3) slabs kt + 2 and
-    // kt + 3 = 9; group 1 (in LOAD kt, having issued kt + 2) that slab = 5 or 4.
-    issue(kb);
-    issue(kb + 1);
-    issue(kb + 2);
-    wait_vmcnt<9>();
+    // Waits.  A wave issues PIECES + 1 loads with an even slab (scales first), PIECES with an odd one, slabs in order.  Before the barrier behind which slab
+    // kt + 1 is read, a wave may still have in flight what it issued after slab kt + 1: group 0 (at the end of MFMA kt, having issued kt + D - 1) the D - 2 slabs
+    // behind it, group 1 (in LOAD kt, having issued kt + D - 2) D - 3 of them, the first of kt's own parity.
+#pragma unroll
+    for (int i = 0; i < D - 1; ++i) issue(kb + i);
+    constexpr int AHEAD0 = (D - 2) * PIECES + (D - 2) / 2, AHEAD1 = (D - 3) * PIECES + (D - 4) / 2;
+    wait_vmcnt<AHEAD0>();
     FP8_BARRIER()
-    // slab kt + 3 goes where slab kt - 1 was: its last readers (group 1, LOAD kt - 1) had their reads done before the barrier that ended that phase
+    // slab kt + D - 1 goes where slab kt - 1 was: its last readers (group 1, LOAD kt - 1) had their reads done before the barrier that ended that phase
     if (grp == 0) {
         for (int kt = kb; kt < nt; kt += 2) {
             load_frags(kt, true);
             FP8_BARRIER()
-            compute_dma(kt + 3, false);
-            wait_vmcnt<9>();
+            compute_dma(kt + D - 1, false);
+            wait_vmcnt<AHEAD0>();
             FP8_BARRIER()
             load_frags(kt + 1, false);
             FP8_BARRIER()
-            compute_dma(kt + 4, true);
-            wait_vmcnt<9>();
+            compute_dma(kt + D, true);
+            wait_vmcnt<AHEAD0>();
             FP8_BARRIER()
         }
         FP8_BARRIER()                                         // slot 2 nt: group 1's last MFMA phase
@@ -619,50 +704,64 @@ __global__ __launch_bounds__(512) void fp8_pingpong_kernel(const Fp8Args g, floa
         FP8_BARRIER()                                         // slot 0
         for (int kt = kb; kt < nt; kt += 2) {
             load_frags(kt, true);
-            wait_vmcnt<5>();
+            wait_vmcnt<AHEAD1 + 1>();
             FP8_BARRIER()
-            compute_dma(kt + 3, false);
+            compute_dma(kt + D - 1, false);
             FP8_BARRIER()
             load_frags(kt + 1, false);
-            wait_vmcnt<4>();
+            wait_vmcnt<AHEAD1>();
             FP8_BARRIER()
-            compute_dma(kt + 4, true);
+            compute_dma(kt + D, true);
             FP8_BARRIER()
         }
     }
     wait_vmcnt<0>();                                          // (every load to LDS has landed before the staging below lies over the ring)
     __syncthreads();
-    out_wave<4>(g, acc, smem + wave * EST, m0 + grp * 128, n0 + q * 64, gridDim.y > 1 ? ws + (long)blockIdx.y * g.M * g.N : nullptr);
+    out_wave<4, NI>(g, acc, smem + wave * EST, m0 + grp * 128, n0 + q * 32 * NI, slices > 1 ? ws + (long)slice * g.M * g.N : nullptr);
 }
 
 // ---- which kernel and how many K slices
-enum { FP8_FEW, FP8_TILE, FP8_PINGPONG };
+enum { FP8_FEW16, FP8_FEW, FP8_TILE, FP8_HALF, FP8_FULL };
 struct Fp8Plan { int kernel, tiles, slices, per; };
 
+// Few rows: the stream kernels; W in slices only where its rows alone leave CUs idle and every wave keeps two blocks or more.
+// Otherwise the cheapest of the three tilings by rounds of the 256 CUs, in us per round measured at K = 4096 (16-bit outputs): 128 x 128 tiles two to a CU 48
+// (30 when one to a CU is all there is), 256 x 128 tiles 41, 256 x 256 tiles 51.  E.g. 4096 x 2048: 48 / 41 / 51 -> 256 x 128 (measured 48.4 / 41.8 /
+// 49.7); 3000 x 3000 (K = 1000): 78 / 82 / 51 -> 256 x 256 (25.1 / 26.8 / 22.0 us); 2048 x 2048 (K = 2048): 30 / 41 / 51 -> 128 x 128 (19.9 / 21.9 / 27.9 us).
+// 128 x 128 tiles that leave CUs idle are cut along K, 8 blocks or more to a slice (a join launch costs what 8 blocks do: 300 x 1000 x 1000 takes
+// 11.9 us whole, 14.6 in two slices), to one workgroup per CU, two where 24 blocks are left to each (256 x 4096 x 25088: 4 slices 48.1, 8 slices 45.9 us).
 Fp8Plan fp8_plan(int64_t M, int64_t N, int64_t Kp) {
-    const int64_t blocks = Kp / 128, t128 = ((M + 127) / 128) * ((N + 127) / 128), t256 = ((M + 255) / 256) * ((N + 255) / 256);
-    int64_t kernel, tiles, want;
+    const int64_t blocks = Kp / 128, one = 1;
+    const int64_t t128 = ((M + 127) / 128) * ((N + 127) / 128), thalf = ((M + 255) / 256) * ((N + 127) / 128), tfull = ((M + 255) / 256) * ((N + 255) / 256);
+    int64_t kernel, tiles, want = 1;
     if (M <= 32) {
-        kernel = FP8_FEW;
-        tiles = (N + 31) / 32;
-        want = min(512 / max(tiles, (int64_t)1), blocks / 8);                 // two workgroups per CU, two blocks or more per wave
-    } else if (t256 >= 192 && blocks >= 1 && Kp <= (1 << 23)) {
-        kernel = FP8_PINGPONG;
-        tiles = t256;
-        want = 1;
+        kernel = M <= 16 ? FP8_FEW16 : FP8_FEW;
+        tiles = M <= 16 ? (N + 15) / 16 : (N + 31) / 32;
+        want = min(256 / max(tiles, one), blocks / (M <= 16 ? 32 : 64));
     } else {
-        kernel = FP8_TILE;
-        tiles = t128;
-        want = min(512 / max(tiles, (int64_t)1), blocks / 4);
+        const int64_t rest = t128 % 512, c128 = t128 / 512 * 48 + (rest == 0 ? 0 : rest <= 256 ? 30 : 48), chalf = (thalf + 255) / 256 * 41, cfull = (tfull + 255) / 256 * 51;
+        const bool big = blocks >= 1 && Kp <= (1 << 23);                      // (32-bit lane offsets inside a tile's 256 rows)
+        if (big && cfull <= c128 && cfull <= chalf) {
+            kernel = FP8_FULL;
+            tiles = tfull;
+        } else if (big && chalf <= c128) {
+            kernel = FP8_HALF;
+            tiles = thalf;
+        } else {
+            kernel = FP8_TILE;
+            tiles = t128;
+            want = min(256 / max(tiles, one), blocks / 8);
+            if (tiles * want <= 256 && blocks / max(2 * want, one) >= 24) want = 512 / max(tiles, one);
+        }
     }
-    const int64_t slices = max(want, (int64_t)1), per = max((blocks + slices - 1) / slices, (int64_t)1);
-    return {(int)kernel, tiles > 0x7fffffff ? -1 : (int)tiles, (int)max((blocks + per - 1) / per, (int64_t)1), (int)per};       // (no empty slice)
+    const int64_t slices = max(want, one), per = max((blocks + slices - 1) / slices, one);
+    return {(int)kernel, tiles * slices > 0x7fffffff ? -1 : (int)tiles, (int)max((blocks + per - 1) / per, one), (int)per};       // (no empty slice)
 }
 
 template <typename K>
 int fp8_launch(K kernel, const Fp8Plan& p, int threads, int smem, const Fp8Args& g, float* ws, hipStream_t s) {
     if (smem > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, smem) != hipSuccess) return SGG_ERR_LAUNCH;
-    hipLaunchKernelGGL(kernel, dim3(p.tiles, p.slices), dim3(threads), smem, s, g, ws, p.per);
+    hipLaunchKernelGGL(kernel, dim3(p.tiles * p.slices), dim3(threads), smem, s, g, ws, p.per, p.slices);
     SGG_CHECK_LAUNCH();
     return SGG_OK;
 }
@@ -718,9 +817,11 @@ extern "C" int sgg_gemm_fp8(const void* A, const void* A_scale, const void* W, c
     hipStream_t s = (hipStream_t)stream;
     const bool wide = out_dtype == SGG_F32;
     int rc;
-    if (p.kernel == FP8_FEW) rc = fp8_launch(fp8_few_rows_kernel<4>, p, 256, 0, g, ws, s);
+    if (p.kernel == FP8_FEW16) rc = fp8_launch(fp8_few16_kernel<3>, p, 1024, 0, g, ws, s);
+    else if (p.kernel == FP8_FEW) rc = fp8_launch(fp8_few_rows_kernel<4>, p, 256, 0, g, ws, s);
     else if (p.kernel == FP8_TILE) rc = wide ? fp8_launch(fp8_tile_kernel<true>, p, 256, 0, g, ws, s) : fp8_launch(fp8_tile_kernel<false>, p, 256, 0, g, ws, s);
-    else rc = wide ? fp8_launch(fp8_pingpong_kernel<true>, p, 512, PP_SMEM, g, ws, s) : fp8_launch(fp8_pingpong_kernel<false>, p, 512, PP_SMEM, g, ws, s);
+    else if (p.kernel == FP8_HALF) rc = wide ? fp8_launch(fp8_pingpong_kernel<true, 1>, p, 512, pp_smem(1), g, ws, s) : fp8_launch(fp8_pingpong_kernel<false, 1>, p, 512, pp_smem(1), g, ws, s);
+    else rc = wide ? fp8_launch(fp8_pingpong_kernel<true, 2>, p, 512, pp_smem(2), g, ws, s) : fp8_launch(fp8_pingpong_kernel<false, 2>, p, 512, pp_smem(2), g, ws, s);
     if (rc != SGG_OK || p.slices == 1) return rc;
     hipLaunchKernelGGL(fp8_join_kernel, dim3((unsigned)((N + 511) / 512), (unsigned)min((M + 3) / 4, (int64_t)1024)), dim3(256), 0, s, g, ws, p.slices);
     SGG_CHECK_LAUNCH();

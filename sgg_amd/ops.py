@@ -1274,7 +1274,7 @@ class Fp8Rows(object):
 def _fp8_empty(M, K, device):
     Kp = (K + FP8_BLOCK - 1) // FP8_BLOCK * FP8_BLOCK
     return Fp8Rows(torch.empty((M, Kp), dtype=torch.float8_e4m3fn, device=device),
-                   torch.empty(_lib.load().sgg_fp8_scale_bytes(M, K), dtype=torch.uint8, device=device), (M, K))
+                   torch.empty((M + 127) // 128 * Kp, dtype=torch.uint8, device=device), (M, K))        # sgg_fp8_scale_bytes(M, K)
 
 
 def quantize_fp8(x, form='rows', colsum=False):
@@ -1332,19 +1332,13 @@ def _dense_layout(t):
 
 def _grad_list(grads, what):
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    dev = _current_device() if grads else None
     for g in grads:
-        _here(g, what)
+        if g.get_device() != dev:
+            _here(g, what)
         if g.layout is not torch.strided:
             raise TypeError('sgg_amd: %s: dense gradients only (got %s)' % (what, g.layout))
     return grads
-
-
-def _tensor_table(ts):
-    """-> (addresses, sizes, type codes, [(start, end, type)] of the memory of each)"""
-    ptr = [t.data_ptr() for t in ts]
-    num = [t.numel() for t in ts]
-    code = [dt(t) for t in ts]
-    return ptr, num, code, [(p, p + n * (4 if c == SGG_F32 else 2), c) for p, n, c in zip(ptr, num, code)]
 
 
 def _clip_call(grads, outs, max_norm, grad_scale):
@@ -1352,21 +1346,29 @@ def _clip_call(grads, outs, max_norm, grad_scale):
     lib = _lib.load()
     norm = torch.empty((), dtype=torch.float32, device='cuda')
     ws = torch.empty(lib.sgg_clip_grads_parts(n), dtype=torch.float64, device='cuda')
-    ptr, num, code, mem = _tensor_table(grads)
-    optr, ocode = ptr, code
+    ptr = optr = [g.data_ptr() for g in grads]
+    num = [g.numel() for g in grads]
+    code = ocode = [_DT.get(g.dtype, -1) for g in grads]
+    if outs is not None and outs is not grads:
+        optr = [o.data_ptr() for o in outs]
+        ocode = [_DT.get(o.dtype, -1) for o in outs]
+    if -1 in code or -1 in ocode:
+        raise TypeError('sgg_amd: clipping: float32 / bfloat16 / float16 tensors only')
     if outs is not None:
         # every tensor is written by workgroups of its own: no two of them may share memory (one given twice would be scaled twice)
-        if outs is not grads:
-            optr, _, ocode, omem = _tensor_table(outs)
-            mem = mem + [o for o, g in zip(omem, mem) if o != g]             # (an output that IS its gradient: in place)
-        mem = sorted(m for m in mem if m[1] > m[0])
-        for a, b in zip(mem, mem[1:]):
-            if b[0] < a[1]:
+        mem = [(p, p + k * (4 if c == SGG_F32 else 2)) for p, k, c in zip(ptr, num, code) if k]
+        if optr is not ptr:                                      # (an output that IS its gradient: in place)
+            mem += [(o, o + k * (4 if d == SGG_F32 else 2)) for p, o, k, c, d in zip(ptr, optr, num, code, ocode) if k and (o != p or c != d)]
+        mem.sort()
+        end = 0
+        for lo, hi in mem:
+            if lo < end:
                 raise ValueError('sgg_amd: clip_grads_: two of the tensors share memory')
-    Ptrs, Longs, Ints = ctypes.c_void_p * n, ctypes.c_int64 * n, ctypes.c_int * n
-    g, d, sizes = Ptrs(*ptr), Ints(*code), Longs(*num)
-    o, od = (None, None) if outs is None else (g, d) if outs is grads else (Ptrs(*optr), Ints(*ocode))
-    _lib.call('sgg_clip_grads', g, o, sizes, d, od, n, float(max_norm), float(grad_scale), ws.data_ptr(), norm.data_ptr(), _stream())
+            end = hi
+    ptrs, ints = ctypes.c_void_p * n, ctypes.c_int * n
+    g, d = ptrs(*ptr), ints(*code)
+    o, od = (None, None) if outs is None else (g, d) if optr is ptr else (ptrs(*optr), ints(*ocode))
+    _lib.call('sgg_clip_grads', g, o, (ctypes.c_int64 * n)(*num), d, od, n, max_norm, grad_scale, ws.data_ptr(), norm.data_ptr(), _stream())
     return norm
 
 
@@ -1374,7 +1376,7 @@ def grad_norm(grads, grad_scale=1.0):
     """|grad_scale| * the L2 norm over every element of the tensors (f32 / bf16 / f16, mixed) -> f32 scalar on the device, no host
     synchronisation.  Squares are added in 64 bits and in a fixed order."""
     grads = [g if _dense_layout(g) else g.contiguous() for g in _grad_list(grads, 'grad_norm')]
-    return _clip_call(grads, None, 0.0, grad_scale)
+    return _clip_call(grads, None, 0.0, float(grad_scale))
 
 
 def clip_grads_(grads, max_norm, grad_scale=1.0, out=None):
@@ -1391,9 +1393,9 @@ def clip_grads_(grads, max_norm, grad_scale=1.0, out=None):
     for g, o in zip(grads, outs):
         if not _dense_layout(g):
             raise ValueError('sgg_amd: clip_grads_: gradient of shape %s has gaps or overlaps (strides %s)' % (tuple(g.shape), tuple(g.stride())))
-        if o is not g and (o.shape != g.shape or o.stride() != g.stride()):
+        if o is not g and (o.shape != g.shape or not (o.stride() == g.stride() or (o.is_contiguous() and g.is_contiguous()))):
             raise ValueError('sgg_amd: clip_grads_: out %s %s for a gradient %s %s' % (tuple(o.shape), tuple(o.stride()), tuple(g.shape), tuple(g.stride())))
-    norm = _clip_call(grads, outs, max_norm, grad_scale)
+    norm = _clip_call(grads, outs, float(max_norm), float(grad_scale))
     if outs:
         torch.autograd.graph.increment_version(outs)          # written through raw pointers
     return norm
