@@ -324,7 +324,11 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(const Fp8Args g, const fl
 __device__ __forceinline__ void tile_and_slice(int tilesM, int tilesN, int& tm, int& tn, int& slice) {
     const int tiles = tilesM * tilesN, logical = xcd_remap(blockIdx.x, gridDim.x);
     slice = logical / tiles;
-    tile_coords_logical(logical - slice * tiles, tilesM, tilesN, tm, tn);
+    // inside a slice, columns of 4 tiles of M at a time (4 against 8 at 7936 x 4096 x 25088: 699 and 714 us; 16: 729)
+    constexpr int GM = 4;
+    const int t = logical - slice * tiles, first = t / (GM * tilesN) * GM, h = min(GM, tilesM - first), in = t - first * tilesN;
+    tm = first + in % h;
+    tn = in / h;
 }
 
 // ---- (1) up to 32 rows of A: a stream of W.  Bound by reading W once (its bytes / the memory's rate); everything else hides behind that.  A workgroup
@@ -445,16 +449,18 @@ __global__ __launch_bounds__(1024) void fp8_few16_kernel(const Fp8Args g, float*
     }
 }
 
-// ---- (2) the middle: tiles of 128 x 128, 4 waves of 64 x 64, one block of 128 per step, K slices while the tiles do not fill the chip.  Two LDS buffers
-// of 32 KiB (two workgroups per CU): while one block is multiplied, the next one's loads are in flight to registers.
+// ---- (2) the middle: tiles of 128 x 128, one workgroup of eight waves per CU: two teams of four (64 x 64 each) take the blocks of 128 in turn, each through
+// two LDS buffers of its own (32 KiB: one block of A and W), and add their sums in LDS at the end.  While one block is multiplied, the next one's loads are
+// in flight to registers.  (Four waves and two workgroups per CU instead: 2048 x 2048 x 2048 19.9 us against 16.4, and twice the partial outputs where K is cut.)
+constexpr int TILE_TEAM = 65536, TILE_SMEM = 2 * TILE_TEAM;
 template <bool WIDE>
-__global__ __launch_bounds__(256) void fp8_tile_kernel(const Fp8Args g, float* __restrict__ ws, int per, int slices) {
-    __shared__ __attribute__((aligned(16))) unsigned char sm[2][2][128 * 128];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+__global__ __launch_bounds__(512) void fp8_tile_kernel(const Fp8Args g, float* __restrict__ ws, int per, int slices) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), team = wave >> 2, tid = threadIdx.x & 255, lane = tid & 63, q = wave & 3;
     int tm, tn, slice;
     tile_and_slice((g.M + 127) / 128, (g.N + 127) / 128, tm, tn, slice);
     const long m0 = (long)tm * 128, n0 = (long)tn * 128;
-    const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64, fr = lane & 31, fh = lane >> 5;
+    const int wm = (q >> 1) * 64, wn = (q & 1) * 64, fr = lane & 31, fh = lane >> 5;
     const int blocks = (int)(g.Kp / 128), b0 = min(slice * per, blocks), b1 = min(b0 + per, blocks);
     const long gA = ((long)g.M + 127) / 128, gW = ((long)g.N + 127) / 128;
     const unsigned *sa = reinterpret_cast<const unsigned*>(g.As) + (long)tm * 32 + fr, *sw = reinterpret_cast<const unsigned*>(g.Ws) + (long)tn * 32 + fr;
@@ -480,20 +486,25 @@ __global__ __launch_bounds__(256) void fp8_tile_kernel(const Fp8Args g, float* _
         ew_n = sw[(long)b * gW * 32];
     };
     f32x16 acc[2][2] = {};
-    if (b0 < b1) fetch(b0);
-    for (int b = b0; b < b1; ++b) {
-        unsigned char *sA = sm[b & 1][0], *sW = sm[b & 1][1];
+    if (b0 + team < b1) fetch(b0 + team);
+    for (int b = b0; b < b1; b += 2) {                       // (the same trips for every wave: a barrier inside)
+        const bool mine = b + team < b1;
+        char *sA = smem + team * TILE_TEAM + ((b - b0) >> 1 & 1) * 32768, *sW = sA + 16384;
+        unsigned ea = 0, ew = 0;
+        if (mine) {
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            *reinterpret_cast<u32x4*>(sA + at[p]) = ra[p];
-            *reinterpret_cast<u32x4*>(sW + at[p]) = rw[p];
+            for (int p = 0; p < 4; ++p) {
+                *reinterpret_cast<u32x4*>(sA + at[p]) = ra[p];
+                *reinterpret_cast<u32x4*>(sW + at[p]) = rw[p];
+            }
+            ea = ea_n >> (wm / 4), ew = ew_n >> (wn / 4);
         }
-        const unsigned ea = ea_n >> (wm / 4), ew = ew_n >> (wn / 4);
-        if (b + 1 < b1) fetch(b + 1);
-        // one barrier per block: this buffer's last readers (block b - 2) passed the barrier of block b - 1 with their reads done
+        if (b + team + 2 < b1) fetch(b + team + 2);
+        // one barrier per step: this buffer's last readers (two steps ago) passed the previous step's barrier with their reads done
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
+        if (!mine) continue;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             i32x8 a[2], w[2];
@@ -517,8 +528,31 @@ __global__ __launch_bounds__(256) void fp8_tile_kernel(const Fp8Args g, float* _
             }
         }
     }
-    __syncthreads();                                          // (the staging below lies over the operand buffers)
-    out_wave<2, 2>(g, acc, reinterpret_cast<char*>(sm) + wave * EST, m0 + wm, n0 + wn, slices > 1 ? ws + (long)slice * g.M * g.N : nullptr);
+    __syncthreads();                                          // (what follows lies over the operand buffers)
+    float* part = slices > 1 ? ws + (long)slice * g.M * g.N : nullptr;
+    // team t keeps the 32 rows mi = t of its wave's tile and hands the other 32 over; (team 0) + (team 1) either way
+    f32x4* give = reinterpret_cast<f32x4*>(smem) + wave * 512 + lane;
+    const f32x4* take = reinterpret_cast<const f32x4*>(smem) + (wave ^ 4) * 512 + lane;
+#pragma unroll
+    for (int ni = 0; ni < 2; ++ni)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const f32x16& o = team ? acc[0][ni] : acc[1][ni];
+            give[(ni * 4 + c) * 64] = f32x4{o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]};
+        }
+    __syncthreads();
+    f32x16 sum[1][2];
+#pragma unroll
+    for (int ni = 0; ni < 2; ++ni)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const f32x4 t = take[(ni * 4 + c) * 64];
+            const f32x16& o = team ? acc[1][ni] : acc[0][ni];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sum[0][ni][4 * c + k] = o[4 * c + k] + t[k];
+        }
+    __syncthreads();
+    out_wave<1, 2>(g, sum, smem + wave * EST, m0 + wm + team * 32, n0 + wn, part);
 }
 
 // ---- (3) large: tiles of 256 x 128 NI, 8 waves = two groups of four, one wave of each group per SIMD; a wave owns 128 x 32 NI.  K advances in slabs of 64
@@ -725,11 +759,11 @@ enum { FP8_FEW16, FP8_FEW, FP8_TILE, FP8_HALF, FP8_FULL };
 struct Fp8Plan { int kernel, tiles, slices, per; };
 
 // Few rows: the stream kernels; W in slices only where its rows alone leave CUs idle and every wave keeps two blocks or more.
-// Otherwise the cheapest of the three tilings by rounds of the 256 CUs, in us per round measured at K = 4096 (16-bit outputs): 128 x 128 tiles two to a CU 48
-// (30 when one to a CU is all there is), 256 x 128 tiles 41, 256 x 256 tiles 51.  E.g. 4096 x 2048: 48 / 41 / 51 -> 256 x 128 (measured 48.4 / 41.8 /
-// 49.7); 3000 x 3000 (K = 1000): 78 / 82 / 51 -> 256 x 256 (25.1 / 26.8 / 22.0 us); 2048 x 2048 (K = 2048): 30 / 41 / 51 -> 128 x 128 (19.9 / 21.9 / 27.9 us).
-// 128 x 128 tiles that leave CUs idle are cut along K, 8 blocks or more to a slice (a join launch costs what 8 blocks do: 300 x 1000 x 1000 takes
-// 11.9 us whole, 14.6 in two slices), to one workgroup per CU, two where 24 blocks are left to each (256 x 4096 x 25088: 4 slices 48.1, 8 slices 45.9 us).
+// Otherwise the cheapest of the three tilings by rounds of the 256 CUs, in us per round measured at K = 4096 (16-bit outputs): 128 x 128 tiles 27, 256 x 128 tiles
+// 41, 256 x 256 tiles 51.  E.g. 1024 x 4096: 27 / 41 / 51 -> 128 x 128 (measured 27.6 / 32.7 / 39.6 us); 4096 x 2048: 54 / 41 / 51 -> 256 x 128 (50.1 / 40.5 /
+// 50.5); 3000 x 3000 (K = 1000): 81 / 82 / 51 -> 256 x 256 (25.1 / 26.8 / 22.0 us).
+// 128 x 128 tiles that leave CUs idle are cut along K, 16 blocks or more to a slice, in two only from 48 blocks on (a join launch costs what some 8 steps do:
+// 512 x 4096 x 4096 takes 25.2 us whole, 27.2 in two slices; 256 x 4096 x 25088 43.9 in four).
 Fp8Plan fp8_plan(int64_t M, int64_t N, int64_t Kp) {
     const int64_t blocks = Kp / 128, one = 1;
     const int64_t t128 = ((M + 127) / 128) * ((N + 127) / 128), thalf = ((M + 255) / 256) * ((N + 127) / 128), tfull = ((M + 255) / 256) * ((N + 255) / 256);
@@ -739,7 +773,7 @@ Fp8Plan fp8_plan(int64_t M, int64_t N, int64_t Kp) {
         tiles = M <= 16 ? (N + 15) / 16 : (N + 31) / 32;
         want = min(256 / max(tiles, one), blocks / (M <= 16 ? 32 : 64));
     } else {
-        const int64_t rest = t128 % 512, c128 = t128 / 512 * 48 + (rest == 0 ? 0 : rest <= 256 ? 30 : 48), chalf = (thalf + 255) / 256 * 41, cfull = (tfull + 255) / 256 * 51;
+        const int64_t c128 = (t128 + 255) / 256 * 27, chalf = (thalf + 255) / 256 * 41, cfull = (tfull + 255) / 256 * 51;
         const bool big = blocks >= 1 && Kp <= (1 << 23);                      // (32-bit lane offsets inside a tile's 256 rows)
         if (big && cfull <= c128 && cfull <= chalf) {
             kernel = FP8_FULL;
@@ -750,8 +784,8 @@ Fp8Plan fp8_plan(int64_t M, int64_t N, int64_t Kp) {
         } else {
             kernel = FP8_TILE;
             tiles = t128;
-            want = min(256 / max(tiles, one), blocks / 8);
-            if (tiles * want <= 256 && blocks / max(2 * want, one) >= 24) want = 512 / max(tiles, one);
+            want = min(256 / max(tiles, one), blocks / 16);
+            if (want == 2 && blocks < 48) want = 1;
         }
     }
     const int64_t slices = max(want, one), per = max((blocks + slices - 1) / slices, one);
@@ -819,7 +853,7 @@ extern "C" int sgg_gemm_fp8(const void* A, const void* A_scale, const void* W, c
     int rc;
     if (p.kernel == FP8_FEW16) rc = fp8_launch(fp8_few16_kernel<3>, p, 1024, 0, g, ws, s);
     else if (p.kernel == FP8_FEW) rc = fp8_launch(fp8_few_rows_kernel<4>, p, 256, 0, g, ws, s);
-    else if (p.kernel == FP8_TILE) rc = wide ? fp8_launch(fp8_tile_kernel<true>, p, 256, 0, g, ws, s) : fp8_launch(fp8_tile_kernel<false>, p, 256, 0, g, ws, s);
+    else if (p.kernel == FP8_TILE) rc = wide ? fp8_launch(fp8_tile_kernel<true>, p, 512, TILE_SMEM, g, ws, s) : fp8_launch(fp8_tile_kernel<false>, p, 512, TILE_SMEM, g, ws, s);
     else if (p.kernel == FP8_HALF) rc = wide ? fp8_launch(fp8_pingpong_kernel<true, 1>, p, 512, pp_smem(1), g, ws, s) : fp8_launch(fp8_pingpong_kernel<false, 1>, p, 512, pp_smem(1), g, ws, s);
     else rc = wide ? fp8_launch(fp8_pingpong_kernel<true, 2>, p, 512, pp_smem(2), g, ws, s) : fp8_launch(fp8_pingpong_kernel<false, 2>, p, 512, pp_smem(2), g, ws, s);
     if (rc != SGG_OK || p.slices == 1) return rc;
