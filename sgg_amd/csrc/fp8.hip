@@ -464,7 +464,7 @@ __global__ __launch_bounds__(512) void fp8_tile_kernel(const Fp8Args g, float* _
     const int blocks = (int)(g.Kp / 128), b0 = min(slice * per, blocks), b1 = min(b0 + per, blocks);
     const long gA = ((long)g.M + 127) / 128, gW = ((long)g.N + 127) / 128;
     const unsigned *sa = reinterpret_cast<const unsigned*>(g.As) + (long)tm * 32 + fr, *sw = reinterpret_cast<const unsigned*>(g.Ws) + (long)tn * 32 + fr;
-    // thread -> rows tid / 8 + 32 p, 16-byte piece tid % 8, stored at the piece permuted by the row (reads of 32 rows then spread over the banks)
+    // thread -> rows tid / 8 + 32 p, 16-byte piece tid % 8, stored at the piece permuted by half the row number (16 rows' reads of one piece then hit every bank once)
     const unsigned char *ap[4], *wp[4];
     int at[4];
 #pragma unroll
@@ -472,7 +472,7 @@ __global__ __launch_bounds__(512) void fp8_tile_kernel(const Fp8Args g, float* _
         const int r = p * 32 + (tid >> 3), h = tid & 7;
         ap[p] = g.A + min(m0 + r, (long)g.M - 1) * g.Kp + h * 16;
         wp[p] = g.W + min(n0 + r, (long)g.N - 1) * g.Kp + h * 16;
-        at[p] = r * 128 + ((h ^ (r & 7)) << 4);
+        at[p] = r * 128 + ((h ^ (r >> 1 & 7)) << 4);
     }
     u32x4 ra[4], rw[4];
     unsigned ea_n = 0, ew_n = 0;
@@ -511,8 +511,8 @@ __global__ __launch_bounds__(512) void fp8_tile_kernel(const Fp8Args g, float* _
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int ra_ = wm + i * 32 + fr, rw_ = wn + i * 32 + fr, h = s * 4 + fh * 2;
-                a[i] = join8(*reinterpret_cast<const u32x4*>(sA + ra_ * 128 + ((h ^ (ra_ & 7)) << 4)), *reinterpret_cast<const u32x4*>(sA + ra_ * 128 + (((h + 1) ^ (ra_ & 7)) << 4)));
-                w[i] = join8(*reinterpret_cast<const u32x4*>(sW + rw_ * 128 + ((h ^ (rw_ & 7)) << 4)), *reinterpret_cast<const u32x4*>(sW + rw_ * 128 + (((h + 1) ^ (rw_ & 7)) << 4)));
+                a[i] = join8(*reinterpret_cast<const u32x4*>(sA + ra_ * 128 + ((h ^ (ra_ >> 1 & 7)) << 4)), *reinterpret_cast<const u32x4*>(sA + ra_ * 128 + (((h + 1) ^ (ra_ >> 1 & 7)) << 4)));
+                w[i] = join8(*reinterpret_cast<const u32x4*>(sW + rw_ * 128 + ((h ^ (rw_ >> 1 & 7)) << 4)), *reinterpret_cast<const u32x4*>(sW + rw_ * 128 + (((h + 1) ^ (rw_ >> 1 & 7)) << 4)));
             }
             if constexpr (WIDE) {
                 const Wide a0 = widen(a[0], scale_f32<0>(ea)), a1 = widen(a[1], scale_f32<1>(ea)), w0 = widen(w[0], scale_f32<0>(ew)), w1 = widen(w[1], scale_f32<1>(ew));

@@ -328,7 +328,11 @@ class _LayerNorm(torch.autograd.Function):
     def backward(ctx, dy):
         x, stats, w = ctx.saved_tensors
         need = ctx.needs_input_grad
-        return ops.layer_norm_bwd(_row_form(dy), x, stats[0], stats[1], w, need[0], need[1], need[2]) + (None,)
+        ops._here(x, 'layer_norm backward')
+        dy = _row_form(dy)                           # (autograd has seen to its shape and type; x and w were checked on the way in)
+        C, mean = x.shape[1], stats.data_ptr()
+        return ops._layer_norm_bwd(dy, max(dy.stride(0), C), x, max(x.stride(0), C), mean, mean + 4 * x.shape[0], None if w is None else w.data_ptr(),
+                                   need[0], need[1], need[2]) + (None,)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):

@@ -1226,6 +1226,24 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, stats=True):
     return (y, st[0], st[1]) if stats else (y, None, None)
 
 
+def _layer_norm_bwd(dy, ld_dy, x, ld, mean, rstd, w, want_dx, want_dw, want_db):
+    """mean, rstd, w: addresses"""
+    M, C = x.shape
+    code = dt(x)
+    dx = torch.empty((M, C), dtype=x.dtype, device=x.device) if want_dx else None
+    dw = torch.empty(C, dtype=torch.float32, device=x.device) if want_dw else None
+    db = torch.empty(C, dtype=torch.float32, device=x.device) if want_db else None
+    ws = None
+    if want_dw or want_db:
+        parts = _lib.load().sgg_layer_norm_bwd_parts(M, C, code)
+        _lib.check(min(parts, 0), 'sgg_layer_norm_bwd_parts')
+        ws = _ws(2 * C * parts, x.device)
+    if want_dx or ws is not None:
+        _lib.call('sgg_layer_norm_bwd', dy.data_ptr(), ld_dy, x.data_ptr(), ld, w, mean, rstd, dx.data_ptr() if want_dx else None,
+                  dw.data_ptr() if want_dw else None, db.data_ptr() if want_db else None, None if ws is None else ws.data_ptr(), M, C, code, _stream())
+    return dx, dw, db
+
+
 def layer_norm_bwd(dy, x, mean, rstd, weight=None, want_dx=True, want_dw=True, want_db=True):
     """the adjoint of layer_norm: dy, x [M, C] of one type, mean / rstd f32[M] as it returned them -> (dx [M, C], dw f32[C], db f32[C]),
     None for what is not wanted.  The sums over the rows are added in a fixed order: same inputs, same bits."""
@@ -1237,17 +1255,7 @@ def layer_norm_bwd(dy, x, mean, rstd, weight=None, want_dx=True, want_dw=True, w
     if not 1 <= C <= LAYER_NORM_MAX:
         raise ValueError('sgg_amd: layer_norm_bwd: rows of 1 .. %d columns, got %d' % (LAYER_NORM_MAX, C))
     mu, r, w = _vector(mean, M, 'layer_norm_bwd mean'), _vector(rstd, M, 'layer_norm_bwd rstd'), _vector(weight, C, 'layer_norm_bwd weight')
-    dx = torch.empty((M, C), dtype=x.dtype, device=x.device) if want_dx else None
-    dw = torch.empty(C, dtype=torch.float32, device=x.device) if want_dw else None
-    db = torch.empty(C, dtype=torch.float32, device=x.device) if want_db else None
-    ws = None
-    if want_dw or want_db:
-        parts = _lib.load().sgg_layer_norm_bwd_parts(M, C, dt(x))
-        _lib.check(min(parts, 0), 'sgg_layer_norm_bwd_parts')
-        ws = _ws(2 * C * parts, x.device)
-    if want_dx or ws is not None:
-        _lib.call('sgg_layer_norm_bwd', dy.data_ptr(), ld_dy, x.data_ptr(), ld, w, mu, r, _p(dx), _p(dw), _p(db), _p(ws), M, C, dt(x), _stream())
-    return dx, dw, db
+    return _layer_norm_bwd(dy, ld_dy, x, ld, mu, r, w, want_dx, want_dw, want_db)
 
 
 class Fp8Rows(object):
