@@ -792,9 +792,13 @@ Fp8Plan fp8_plan(int64_t M, int64_t N, int64_t Kp) {
     return {(int)kernel, tiles * slices > 0x7fffffff ? -1 : (int)tiles, (int)max((blocks + per - 1) / per, one), (int)per};       // (no empty slice)
 }
 
-template <typename K>
-int fp8_launch(K kernel, const Fp8Plan& p, int threads, int smem, const Fp8Args& g, float* ws, hipStream_t s) {
-    if (smem > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, smem) != hipSuccess) return SGG_ERR_LAUNCH;
+template <auto kernel>
+int fp8_launch(const Fp8Plan& p, int threads, int smem, const Fp8Args& g, float* ws, hipStream_t s) {
+    static bool attr_done = false;
+    if (smem > 65536 && !attr_done) {
+        if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, smem) != hipSuccess) return SGG_ERR_LAUNCH;
+        attr_done = true;
+    }
     hipLaunchKernelGGL(kernel, dim3(p.tiles * p.slices), dim3(threads), smem, s, g, ws, p.per, p.slices);
     SGG_CHECK_LAUNCH();
     return SGG_OK;
@@ -851,11 +855,13 @@ extern "C" int sgg_gemm_fp8(const void* A, const void* A_scale, const void* W, c
     hipStream_t s = (hipStream_t)stream;
     const bool wide = out_dtype == SGG_F32;
     int rc;
-    if (p.kernel == FP8_FEW16) rc = fp8_launch(fp8_few16_kernel<3>, p, 1024, 0, g, ws, s);
-    else if (p.kernel == FP8_FEW) rc = fp8_launch(fp8_few_rows_kernel<4>, p, 256, 0, g, ws, s);
-    else if (p.kernel == FP8_TILE) rc = wide ? fp8_launch(fp8_tile_kernel<true>, p, 512, TILE_SMEM, g, ws, s) : fp8_launch(fp8_tile_kernel<false>, p, 512, TILE_SMEM, g, ws, s);
-    else if (p.kernel == FP8_HALF) rc = wide ? fp8_launch(fp8_pingpong_kernel<true, 1>, p, 512, pp_smem(1), g, ws, s) : fp8_launch(fp8_pingpong_kernel<false, 1>, p, 512, pp_smem(1), g, ws, s);
-    else rc = wide ? fp8_launch(fp8_pingpong_kernel<true, 2>, p, 512, pp_smem(2), g, ws, s) : fp8_launch(fp8_pingpong_kernel<false, 2>, p, 512, pp_smem(2), g, ws, s);
+    switch (p.kernel) {
+        case FP8_FEW16: rc = fp8_launch<fp8_few16_kernel<3>>(p, 1024, 0, g, ws, s); break;
+        case FP8_FEW: rc = fp8_launch<fp8_few_rows_kernel<4>>(p, 256, 0, g, ws, s); break;
+        case FP8_TILE: rc = wide ? fp8_launch<fp8_tile_kernel<true>>(p, 512, TILE_SMEM, g, ws, s) : fp8_launch<fp8_tile_kernel<false>>(p, 512, TILE_SMEM, g, ws, s); break;
+        case FP8_HALF: rc = wide ? fp8_launch<fp8_pingpong_kernel<true, 1>>(p, 512, pp_smem(1), g, ws, s) : fp8_launch<fp8_pingpong_kernel<false, 1>>(p, 512, pp_smem(1), g, ws, s); break;
+        default: rc = wide ? fp8_launch<fp8_pingpong_kernel<true, 2>>(p, 512, pp_smem(2), g, ws, s) : fp8_launch<fp8_pingpong_kernel<false, 2>>(p, 512, pp_smem(2), g, ws, s); break;
+    }
     if (rc != SGG_OK || p.slices == 1) return rc;
     hipLaunchKernelGGL(fp8_join_kernel, dim3((unsigned)((N + 511) / 512), (unsigned)min((M + 3) / 4, (int64_t)1024)), dim3(256), 0, s, g, ws, p.slices);
     SGG_CHECK_LAUNCH();

@@ -177,15 +177,22 @@ def affine_fp8(x, weight, bias=None, out_dtype=None):
     """x [..., K] (f32 / bf16 / f16) -> [..., N] = x . weight^T + bias in 8-bit floating point (ops.gemm_fp8), out_dtype (default x's type);
     differentiable in all three, the gradients' products in 8 bits too.  What set_compute('fp8') makes of affine / conv2d."""
     _need_gpu(x)
-    y = _AffineFp8.apply(x.reshape(-1, x.shape[-1]), weight, bias, out_dtype or x.dtype)
-    return y.view(*x.shape[:-1], weight.shape[0])
+    return _affine_fp8_rows(x.reshape(-1, x.shape[-1]), weight, bias, out_dtype or x.dtype).view(*x.shape[:-1], weight.shape[0])
+
+
+def _affine_fp8_rows(x, w, b, out_dtype):
+    if torch.is_grad_enabled():
+        return _AffineFp8.apply(x, w, b, out_dtype)
+    if x.shape[1] != w.shape[1]:
+        raise ValueError('dense: inputs %s against weights %s' % (tuple(x.shape), tuple(w.shape)))
+    return ops.gemm_fp8(ops.quantize_fp8(_row_form(x)), ops.quantize_fp8(_row_form(w)), b.detach().float().contiguous() if b is not None else None, out_dtype=out_dtype)
 
 
 def _affine_rows(x, w, b):
     """the product of a row matrix in the file's arithmetic (columns of x past w's are zero: a padded patch matrix)"""
     if _COMPUTE[0] != 'fp8':
         return _Affine.apply(x, w, b)
-    return _AffineFp8.apply(x, w if w.shape[1] == x.shape[1] else F.pad(w, (0, x.shape[1] - w.shape[1])), b, torch.float32)
+    return _affine_fp8_rows(x, w if w.shape[1] == x.shape[1] else F.pad(w, (0, x.shape[1] - w.shape[1])), b, torch.float32)
 
 
 def affine(x, weight, bias=None):

@@ -1178,9 +1178,10 @@ _current_device = getattr(torch._C, '_cuda_getDevice', None) or torch.cuda.curre
 
 def _here(t, what):
     """the launch goes to the current device's stream: a tensor of another device is refused, not run there"""
-    if t.get_device() != _current_device():
-        if not t.is_cuda:
-            raise RuntimeError('sgg_amd: %s: tensor is not on the GPU (the HIP path has no CPU fallback)' % what)
+    d = t.get_device()
+    if d < 0:
+        raise RuntimeError('sgg_amd: %s: tensor is not on the GPU (the HIP path has no CPU fallback)' % what)
+    if d != _current_device():
         raise RuntimeError('sgg_amd: %s: tensor is on %s, the current device is cuda:%d' % (what, t.device, _current_device()))
 
 
@@ -1315,8 +1316,13 @@ def gemm_fp8(A, W, bias=None, act=ACT_NONE, out_dtype=torch.float32, out=None):
     (M, K), N = A.shape, W.shape[0]
     if W.shape[1] != K:
         raise ValueError('sgg_amd: gemm_fp8: %s . %s^T' % (A.shape, W.shape))
-    for t in (A.data, A.scale, W.data, W.scale):
-        _here(t, 'gemm_fp8')
+    for q in (A, W):
+        d, sc, (rows, cols) = q.data, q.scale, q.shape
+        _here(d, 'gemm_fp8')
+        _here(sc, 'gemm_fp8')
+        Kp = (cols + FP8_BLOCK - 1) // FP8_BLOCK * FP8_BLOCK
+        if d.dtype != torch.float8_e4m3fn or sc.dtype != torch.uint8 or d.shape != (rows, Kp) or sc.numel() != (rows + 127) // 128 * Kp:
+            raise ValueError('sgg_amd: gemm_fp8: operand [%d, %d] holds %s %s and %d scales' % (rows, cols, d.dtype, tuple(d.shape), sc.numel()))
     b = _vector(bias, N, 'gemm_fp8 bias')
     if out is None:
         out = torch.empty((M, N), dtype=out_dtype, device=A.data.device)
@@ -1325,7 +1331,6 @@ def gemm_fp8(A, W, bias=None, act=ACT_NONE, out_dtype=torch.float32, out=None):
         if tuple(out.shape) != (M, N):
             raise ValueError('sgg_amd: gemm_fp8: out %s for a [%d, %d] product' % (tuple(out.shape), M, N))
     ldc, code = _row_matrix(out, 'gemm_fp8 out'), dt(out)
-    Kp = A.data.shape[1]
     splits = _lib.load().sgg_gemm_fp8_splits(M, N, Kp)
     _lib.check(min(splits, 0), 'sgg_gemm_fp8_splits')
     ws = _ws(splits * M * N, out.device) if splits > 1 else None
@@ -1334,16 +1339,24 @@ def gemm_fp8(A, W, bias=None, act=ACT_NONE, out_dtype=torch.float32, out=None):
 
 
 def _dense_layout(t):
-    """elements fill one memory range (whatever the order of the axes)"""
-    return t.is_contiguous() or (t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last))
+    """the elements fill one memory range, whatever the order of the axes"""
+    if t.is_contiguous():
+        return True
+    step = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != step:
+            return False
+        step *= size
+    return True
 
 
 def _grad_list(grads, what):
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-    dev = _current_device() if grads else None
+    dev = None
     for g in grads:
-        if g.get_device() != dev:
+        if g.get_device() != dev or dev is None:
             _here(g, what)
+            dev = g.get_device()
         if g.layout is not torch.strided:
             raise TypeError('sgg_amd: %s: dense gradients only (got %s)' % (what, g.layout))
     return grads

@@ -116,6 +116,8 @@ def test_parameters_form_follows_torch():
         if i != 5:
             p.grad = torch.randn_like(p)
     net[0].weight.grad = net[0].weight.grad.contiguous(memory_format=torch.channels_last)      # dense in another order
+    net.register_parameter('turned', torch.nn.Parameter(torch.randn(6, 7, 5, device=DEV).permute(2, 0, 1)))
+    net.turned.grad = torch.randn(6, 7, 5, device=DEV).permute(2, 0, 1)
     grads = [p.grad for p in net.parameters() if p.grad is not None]
     want = want_of(grads, 2.0)
     check(clip_grad_norm_(net.parameters(), 2.0), grads, want)

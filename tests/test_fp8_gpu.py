@@ -63,6 +63,38 @@ def test_operand_form_is_the_definition(M, K, dtype):
     assert torch.equal(alone_t.data.view(torch.uint8), c.data.view(torch.uint8)) and torch.equal(alone_t.scale, c.scale)
 
 
+@pytest.mark.parametrize('dtype,bits', [(F32, 0x7f800001), (F32, -0x7fffff), (F16, 0x7c01), (BF16, 0x7f81)])
+def test_signalling_nan_changes_nothing_but_itself(dtype, bits):
+    from sgg_amd import ops
+    x = rand(130, 140, dtype, 2)
+    ref = [q.dequantize() for q in ops.quantize_fp8(x, 'both')]
+    x.view(torch.int32 if dtype == F32 else torch.int16)[7, 9] = bits
+    x0 = x.clone()
+    x0[7, 9] = 0
+    for q, r, z in zip(ops.quantize_fp8(x, 'both'), ref, ops.quantize_fp8(x0, 'both')):
+        v, w = q.dequantize(), z.dequantize()
+        at = (7, 9) if v.shape[0] == 130 else (9, 7)
+        assert bool(v[at].isnan()) and int(v.isnan().sum()) == 1 and torch.equal(q.exponents(), z.exponents())
+        v[at] = w[at]
+        assert torch.equal(v, w)
+
+
+def test_column_sums_ride_along():
+    """quantize_fp8(colsum=True): f32 sums of 128 rows at a time, then of the tiles: off by (rows + 8) half steps of the sum of magnitudes"""
+    from sgg_amd import ops
+    for M, K, dtype in ((1, 5, F32), (700, 300, BF16), (1300, 130, F16), (0, 7, F32)):
+        x = rand(M, K, dtype, M, 0.5)
+        for form in ('cols', 'both'):
+            q, sums = ops.quantize_fp8(x, form, colsum=True)
+            assert sums.shape == (K,) and sums.dtype == F32
+            assert float(((sums.double() - x.double().sum(0)).abs() - (M + 8) * U * x.double().abs().sum(0)).max()) <= 0
+            plain = ops.quantize_fp8(x, form)
+            for a, b in zip(q if form == 'both' else (q,), plain if form == 'both' else (plain,)):
+                assert torch.equal(a.data.view(torch.uint8), b.data.view(torch.uint8)) and torch.equal(a.scale, b.scale)
+    with pytest.raises(ValueError):
+        ops.quantize_fp8(rand(3, 4, F32, 1), colsum=True)
+
+
 def test_every_code_ties_extremes_and_non_finite():
     from sgg_amd import ops
     codes = torch.arange(256, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn).float()
@@ -121,7 +153,10 @@ def check(got, want, tol):
 
 SIZES = [(1, 1, 1), (1, 128, 128), (2, 100, 5), (1, 4096, 1000), (3, 25088, 300), (16, 1000, 4096), (17, 640, 33), (31, 3000, 100), (32, 2048, 512),
          (33, 1100, 129), (64, 5000, 64), (100, 4096, 700), (128, 128, 128), (127, 257, 129), (256, 12544, 256), (256, 640, 512), (300, 1024, 300),
-         (513, 512, 257), (1000, 384, 1000), (1985, 1100, 333), (2048, 896, 2048), (2304, 640, 2300), (4097, 256, 260), (5000, 130, 3), (7, 130, 5000)]
+         (513, 512, 257), (1000, 384, 1000), (1985, 1100, 333), (2048, 896, 2048), (2304, 640, 2300), (4097, 256, 260), (5000, 130, 3), (7, 130, 5000),
+         (24, 25088, 300), (40, 25088, 300), (300, 12544, 200),                        # K slices of each kind
+         (2304, 100, 2300), (2500, 1000, 2450), (2561, 129, 2000),                     # 256 x 128 tiles: one block, several, ragged edges
+         (3000, 100, 3000), (3001, 256, 2901), (3000, 385, 3000), (4352, 700, 4500), (2816, 2048, 3328)]   # 256 x 256 tiles
 
 
 @pytest.mark.parametrize('out', [F32, F16, BF16])
@@ -211,6 +246,14 @@ def test_affine_forward_and_gradients(M, K, N, dtype):
     y3 = dense.affine_fp8(x, w.detach(), b.detach())
     assert torch.equal(torch.autograd.grad(y3, x, dy)[0], dx)
     assert torch.equal(dense.affine_fp8(x.detach().view(1, M, K), w.detach(), b.detach(), out_dtype=dtype).view(M, N), y.detach())
+    with torch.no_grad():
+        assert torch.equal(dense.affine_fp8(x, w, b), y)
+    # a gradient that autograd hands over as one broadcast number, transposed weights, strided inputs
+    ys = dense.affine_fp8(x, w.t().contiguous().t(), b)
+    assert torch.equal(ys, y)
+    gs = torch.autograd.grad(ys.sum(), (x, w, b))
+    gf = torch.autograd.grad(dense.affine_fp8(x, w, b), (x, w, b), torch.ones_like(dy))
+    assert all(torch.equal(p, q) for p, q in zip(gs, gf))
 
 
 def test_relative_error_against_the_unquantised_product():
@@ -254,7 +297,7 @@ def test_dense_layers_in_the_fp8_arithmetic():
     dw = torch.mm(quant(dhm.t()), quant(cols.t()).t().contiguous())[:, :81].view(12, 3, 3, 9).permute(0, 3, 1, 2)
     assert float((grads[1].double() - dw).abs().max()) <= 200 * U * float(dhm.abs().sum(0).max() * cols.abs().max())
     dl = torch.mm(quant(dym.t()), quant(h.detach().reshape(60, 12).t()).t().contiguous())
-    assert float((grads[3].double() - dl).abs().max()) <= 200 * U * float(dym.abs().sum(0).max() * h.abs().max())
+    assert float((grads[3].double() - dl).abs().max()) <= 200 * U * float((dym.abs().sum(0).max() * h.abs().max()).detach())
     assert grads[0].shape == x.shape and grads[2].shape == (12,) and grads[4].shape == (7,)
 
 
@@ -342,6 +385,10 @@ def test_refusals():
         ops.gemm_fp8(x, A)
     with pytest.raises(ValueError):
         ops.gemm_fp8(A, ops.quantize_fp8(x[:, :255]))                     # same padded width, another reduction
+    for bad in (ops.Fp8Rows(A.data[:3], A.scale, (4, 256)), ops.Fp8Rows(A.data, A.scale[:100], (4, 256)), ops.Fp8Rows(A.data, A.scale, (4, 300)),
+                ops.Fp8Rows(A.data.view(torch.uint8), A.scale, (4, 256))):
+        with pytest.raises(ValueError):                                   # an operand whose memory is not its shape's
+            ops.gemm_fp8(bad, bad)
     with pytest.raises(ValueError):
         ops.gemm_fp8(A, A, torch.zeros(5, device=DEV))
     with pytest.raises(TypeError):

@@ -185,6 +185,23 @@ def test_gradients_against_differences():
         assert abs(float((g.double() * d).sum() - want)) <= 100 * U * float((g.double() * d).abs().sum()) + 1e-6
 
 
+def test_broadcast_gradients_and_another_stream():
+    from sgg_amd import dense
+    torch.manual_seed(6)
+    for shape in ((5, 7), (4, 1), (1, 9)):
+        m = dense.LayerNormRows(shape[1]).to(DEV)
+        x = torch.randn(shape, device=DEV, requires_grad=True)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            a = torch.autograd.grad(m(x).sum(), (x, m.weight, m.bias))             # dy: one number, strides 0
+        s.synchronize()
+        b = torch.autograd.grad(m(x), (x, m.weight, m.bias), torch.ones(shape, device=DEV))
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+    x = torch.randn(3, 4, 10, device=DEV, requires_grad=True)
+    assert torch.equal(dense.layer_norm(x.transpose(0, 1)[..., :8]), dense.layer_norm(x.detach().transpose(0, 1)[..., :8].contiguous()))
+
+
 def test_graph_convolution_net_with_layer_norm_trains():
     """build_mlp(batch_norm='layer'): the scene-graph convolutions run forward and backward through it, every parameter gets a gradient"""
     from sgg_amd import dense
