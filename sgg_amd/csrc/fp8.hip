@@ -575,7 +575,7 @@ __device__ __forceinline__ void lds_piece(const char* ubase, unsigned& off, char
 
 constexpr int PP_ROW = 64;
 constexpr int pp_stage(int NI) { return (256 + 128 * NI) * PP_ROW; }
-constexpr int PP_DEPTH = 4;                                           // slabs of the ring (even; 6 measured no faster)
+constexpr int PP_DEPTH = 4;                                           // slabs of the ring (a power of two; 6 measured no faster)
 constexpr int pp_smem(int NI) { return PP_DEPTH * pp_stage(NI) + 4 * 8 * 256; }
 
 template <bool WIDE, int NI>
@@ -620,7 +620,7 @@ __global__ __launch_bounds__(512) void fp8_pingpong_kernel(const Fp8Args g, floa
     auto slab_off = [&](int kt) { return (long)min(kt, nt - 1) * PP_ROW; };
     auto issue = [&](int kt) {
         const long k = slab_off(kt);
-        char* dst = smem + (kt % D) * PP_STAGE + lds_rows0;
+        char* dst = smem + (kt & (D - 1)) * PP_STAGE + lds_rows0;
         if (!(kt & 1)) issue_scales(kt);
         lds_piece<0>(uniform_ptr(base_0 + k), vo_0, dst);
         lds_piece<1024>(uniform_ptr(base_1 + k), vo_1, dst);
@@ -637,32 +637,53 @@ __global__ __launch_bounds__(512) void fp8_pingpong_kernel(const Fp8Args g, floa
     i32x8 af[4], wf[NI];
     Wide aw[4], ww[NI];
     unsigned ea = 0, ew = 0;
-    auto load_frags = [&](int kt, bool even) {
+    // addresses of the next slab to read and of the next one to load, made while the matrix pipe is still busy with the last instructions of a phase
+    unsigned ra0, ra1, rw0, rw1, rs, dst;
+    const char *u0, *u1, *u2, *u3;
+    auto prepare = [&](int kt) {
+        const unsigned st = (kt & (D - 1)) * PP_STAGE;
+        ra0 = at_a + st, ra1 = ra0 ^ 32, rw0 = at_w + st, rw1 = rw0 ^ 32;
+        rs = at_s + ((kt >> 1) & 3) * 2048;
+        const long k = slab_off(kt + D - 1);
+        u0 = uniform_ptr(base_0 + k), u1 = uniform_ptr(base_1 + k), u2 = uniform_ptr(base_2 + k), u3 = uniform_ptr(base_3 + k);
+        dst = ((kt + D - 1) & (D - 1)) * PP_STAGE + lds_rows0;
+    };
+    auto load_frags = [&](bool even) {
         // one asm block, with its wait: the compiler waits for EVERY load to LDS in flight before an LDS read of its own
-        const unsigned st = (kt % D) * PP_STAGE;
-        const unsigned a0 = at_a + st, a1 = a0 ^ 32, w0 = at_w + st, w1 = w0 ^ 32;
         u32x4 f[12];
-        // outputs 0 .. 7 the fragments of A, 8 .. 11 those of W; inputs: A's two addresses, W's two
+        unsigned e = 0;
+        // outputs 0 .. 7 the fragments of A, 8 .. the one or two of W, with a block's first slab two words of scales
 #define FP8_READS_A(a0, a1)                                                                                                                    \
     "ds_read_b128 %0, " a0 "\n ds_read_b128 %1, " a1 "\n ds_read_b128 %2, " a0 " offset:2048\n ds_read_b128 %3, " a1 " offset:2048\n"         \
     "ds_read_b128 %4, " a0 " offset:4096\n ds_read_b128 %5, " a1 " offset:4096\n ds_read_b128 %6, " a0 " offset:6144\n ds_read_b128 %7, " a1 " offset:6144\n"
+#define FP8_OUT_A "=&v"(f[0]), "=&v"(f[1]), "=&v"(f[2]), "=&v"(f[3]), "=&v"(f[4]), "=&v"(f[5]), "=&v"(f[6]), "=&v"(f[7]), "=&v"(f[8]), "=&v"(f[9])
         if constexpr (NI == 2) {
-            asm volatile("ds_read_b128 %8, %14\n ds_read_b128 %9, %15\n ds_read_b128 %10, %14 offset:2048\n ds_read_b128 %11, %15 offset:2048\n" FP8_READS_A("%12", "%13") "s_waitcnt lgkmcnt(0)"
-                         : "=&v"(f[0]), "=&v"(f[1]), "=&v"(f[2]), "=&v"(f[3]), "=&v"(f[4]), "=&v"(f[5]), "=&v"(f[6]), "=&v"(f[7]), "=&v"(f[8]), "=&v"(f[9]), "=&v"(f[10]), "=&v"(f[11])
-                         : "v"(a0), "v"(a1), "v"(w0), "v"(w1)
-                         : "memory");
+            if (even)
+                asm volatile("ds_read_b32 %12, %18\n ds_read_b32 %13, %18 offset:128\n"
+                             "ds_read_b128 %8, %16\n ds_read_b128 %9, %17\n ds_read_b128 %10, %16 offset:2048\n ds_read_b128 %11, %17 offset:2048\n" FP8_READS_A("%14", "%15") "s_waitcnt lgkmcnt(0)"
+                             : FP8_OUT_A, "=&v"(f[10]), "=&v"(f[11]), "=&v"(ea), "=&v"(e)
+                             : "v"(ra0), "v"(ra1), "v"(rw0), "v"(rw1), "v"(rs)
+                             : "memory");
+            else
+                asm volatile("ds_read_b128 %8, %14\n ds_read_b128 %9, %15\n ds_read_b128 %10, %14 offset:2048\n ds_read_b128 %11, %15 offset:2048\n" FP8_READS_A("%12", "%13") "s_waitcnt lgkmcnt(0)"
+                             : FP8_OUT_A, "=&v"(f[10]), "=&v"(f[11])
+                             : "v"(ra0), "v"(ra1), "v"(rw0), "v"(rw1)
+                             : "memory");
         } else {
-            asm volatile("ds_read_b128 %8, %12\n ds_read_b128 %9, %13\n" FP8_READS_A("%10", "%11") "s_waitcnt lgkmcnt(0)"
-                         : "=&v"(f[0]), "=&v"(f[1]), "=&v"(f[2]), "=&v"(f[3]), "=&v"(f[4]), "=&v"(f[5]), "=&v"(f[6]), "=&v"(f[7]), "=&v"(f[8]), "=&v"(f[9])
-                         : "v"(a0), "v"(a1), "v"(w0), "v"(w1)
-                         : "memory");
+            if (even)
+                asm volatile("ds_read_b32 %10, %16\n ds_read_b32 %11, %16 offset:128\n ds_read_b128 %8, %14\n ds_read_b128 %9, %15\n" FP8_READS_A("%12", "%13") "s_waitcnt lgkmcnt(0)"
+                             : FP8_OUT_A, "=&v"(ea), "=&v"(e)
+                             : "v"(ra0), "v"(ra1), "v"(rw0), "v"(rw1), "v"(rs)
+                             : "memory");
+            else
+                asm volatile("ds_read_b128 %8, %12\n ds_read_b128 %9, %13\n" FP8_READS_A("%10", "%11") "s_waitcnt lgkmcnt(0)"
+                             : FP8_OUT_A
+                             : "v"(ra0), "v"(ra1), "v"(rw0), "v"(rw1)
+                             : "memory");
         }
 #undef FP8_READS_A
-        if (even) {
-            unsigned e;
-            asm volatile("ds_read_b32 %0, %2\n ds_read_b32 %1, %2 offset:128\n s_waitcnt lgkmcnt(0)" : "=&v"(ea), "=&v"(e) : "v"(at_s + ((kt >> 1) & 3) * 2048) : "memory");
-            ew = e >> (q * NI * 8 & 31);                       // bytes: the wave's NI rows-of-32 inside the group of 128
-        }
+#undef FP8_OUT_A
+        if (even) ew = e >> (q * NI * 8 & 31);                 // bytes: the wave's NI rows-of-32 inside the group of 128
         wf[0] = join8(f[8], f[9]);
         if constexpr (NI == 2) wf[NI - 1] = join8(f[10], f[11]);
 #pragma unroll
@@ -683,25 +704,25 @@ __global__ __launch_bounds__(512) void fp8_pingpong_kernel(const Fp8Args g, floa
         acc[mi][0] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[0], af[mi], acc[mi][0], 0, 0, 0, ew, mi, ea);                             \
         if constexpr (NI == 2) acc[mi][NI - 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[NI - 1], af[mi], acc[mi][NI - 1], 0, 0, 1, ew, mi, ea); \
     }
-    auto compute_dma = [&](int pf, bool scales) {             // the slab's matrix instructions with the loads of slab pf between them
-        const long k = slab_off(pf);
-        const char *u0 = uniform_ptr(base_0 + k), *u1 = uniform_ptr(base_1 + k), *u2 = uniform_ptr(base_2 + k), *u3 = uniform_ptr(base_3 + k);
-        char* dst = smem + (pf % D) * PP_STAGE + lds_rows0;
-        if (scales) issue_scales(pf);
+    auto compute_dma = [&](int kt, bool scales) {             // slab kt's matrix instructions with the loads of slab kt + D - 1 between them
+        char* to = smem + dst;
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_setprio(1);
         FP8_MMA(0)
-        lds_piece<0>(u0, vo_0, dst);
+        if (scales) issue_scales(kt + D - 1);
+        lds_piece<0>(u0, vo_0, to);
         __builtin_amdgcn_sched_barrier(0);
         FP8_MMA(1)
-        lds_piece<1024>(u1, vo_1, dst);
+        lds_piece<1024>(u1, vo_1, to);
         __builtin_amdgcn_sched_barrier(0);
         FP8_MMA(2)
-        lds_piece<2048>(u2, vo_2, dst);
+        lds_piece<2048>(u2, vo_2, to);
         __builtin_amdgcn_sched_barrier(0);
         FP8_MMA(3)
-        if constexpr (NI == 2) lds_piece<3072>(u3, vo_3, dst);
+        if constexpr (NI == 2) lds_piece<3072>(u3, vo_3, to);
         __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+        prepare(kt + 1);
         __builtin_amdgcn_sched_barrier(0);
     };
 #undef FP8_MMA
@@ -720,16 +741,17 @@ __global__ __launch_bounds__(512) void fp8_pingpong_kernel(const Fp8Args g, floa
     wait_vmcnt<AHEAD0>();
     FP8_BARRIER()
     // slab kt + D - 1 goes where slab kt - 1 was: its last readers (group 1, LOAD kt - 1) had their reads done before the barrier that ended that phase
+    prepare(kb);
     if (grp == 0) {
         for (int kt = kb; kt < nt; kt += 2) {
-            load_frags(kt, true);
+            load_frags(true);
             FP8_BARRIER()
-            compute_dma(kt + D - 1, false);
+            compute_dma(kt, false);
             wait_vmcnt<AHEAD0>();
             FP8_BARRIER()
-            load_frags(kt + 1, false);
+            load_frags(false);
             FP8_BARRIER()
-            compute_dma(kt + D, true);
+            compute_dma(kt + 1, true);
             wait_vmcnt<AHEAD0>();
             FP8_BARRIER()
         }
@@ -737,15 +759,15 @@ __global__ __launch_bounds__(512) void fp8_pingpong_kernel(const Fp8Args g, floa
     } else {
         FP8_BARRIER()                                         // slot 0
         for (int kt = kb; kt < nt; kt += 2) {
-            load_frags(kt, true);
+            load_frags(true);
             wait_vmcnt<AHEAD1 + 1>();
             FP8_BARRIER()
-            compute_dma(kt + D - 1, false);
+            compute_dma(kt, false);
             FP8_BARRIER()
-            load_frags(kt + 1, false);
+            load_frags(false);
             wait_vmcnt<AHEAD1>();
             FP8_BARRIER()
-            compute_dma(kt + D, true);
+            compute_dma(kt + 1, true);
             FP8_BARRIER()
         }
     }
