@@ -22,7 +22,7 @@
 extern "C" {
 #endif
 
-#define SGG_ABI_VERSION 16   /* bump whenever a prototype below changes: tests/abi.lock pins (version, digest of the prototypes) */
+#define SGG_ABI_VERSION 17   /* bump whenever a prototype below changes: tests/abi.lock pins (version, digest of the prototypes) */
 
 enum { SGG_F32 = 0, SGG_BF16 = 1, SGG_F16 = 2,
        /* a PAIR of f16 planes x = hi + lo (hi = f16(x), lo = f16(x - hi): 22 significand bits) -- the operand / activation format of the x3
@@ -416,10 +416,11 @@ int sgg_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ldx
                        float* dw, float* db, float* ws, int64_t M, int C, int dtype, void* stream);
 
 /* ---- matrix product in 8-bit floating point (OCP e4m3) with a power-of-two scale for each block of 128 along the reduction ----
- * Operand form of x [M, K]: `rows` u8 [M][Kp], Kp = K rounded up to 128 (zeros past K), and rows_scale u8 [sgg_fp8_scale_bytes(M, K)]: the
- * exponent byte e + 127 of each row and block, e >= -126 the smallest with max|x| <= 448 * 2^e over the block's finite elements (non-finite
- * elements become NaN); byte ((b * G + m / 128) * 32 + m % 32) * 4 + (m / 32) % 4, G = ceil(M / 128).  `cols` / cols_scale: the same form of x^T
- * ([K][Mp]), out of the same reading of x.  Either form may be NULL (with its scales).  rows, cols 16-byte aligned, the scales 4-byte.
+ * Operand form of x [M, K]: `rows` u8 [Kp / 64][R][64], Kp = K rounded up to 128 (zeros past K), R = M rounded up to even (zeros past M): slabs of 64
+ * columns, so that the rows of a tile are contiguous; and rows_scale u8 [sgg_fp8_scale_bytes(M, K)]: the exponent byte e + 127 of each row and
+ * block of 128 columns, e >= -126 the smallest with max|x| <= 448 * 2^e over the block's finite elements (non-finite elements become NaN);
+ * byte ((b * G + m / 128) * 32 + m % 32) * 4 + (m / 32) % 4, G = ceil(M / 128).  `cols` / cols_scale: the same form of x^T, out of the same
+ * reading of x.  Either form may be NULL (with its scales).  rows, cols 16-byte aligned, the scales 4-byte.
  * colsum f32[K] (or NULL; only with `cols`): the column sums of x (a bias gradient of x = dY), added in a fixed order; colsum_ws
  * f32[ceil(M / 128) * K] then.
  * gemm_fp8: C[m][n] = act(sum_k A[m][k] W[n][k] + bias[n]), fp32 accumulation, one rounding to out_dtype; bias f32[N] or NULL; ldc in

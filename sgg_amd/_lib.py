@@ -12,7 +12,7 @@ LIB_PATH = os.environ.get('SGG_HIP_LIB') or os.path.join(_HERE, 'libsgg_hip.so')
 
 SGG_F32, SGG_BF16, SGG_F16 = 0, 1, 2
 ACT_NONE, ACT_RELU = 0, 1
-ABI_VERSION = 16
+ABI_VERSION = 17
 
 import threading  # noqa: E402
 # held by sgg_amd.graph_step while it captures a hipGraph, and by every other thread of this package around its own GPU calls (the

@@ -1,8 +1,10 @@
 // Matrix products in 8-bit floating point (OCP e4m3) with a power-of-two scale for each block of 128 along the reduction.
 //
-// Operand form: row m of a matrix [M][K] is Kp = K rounded up to 128 bytes of e4m3 (zero past K); block b of it, columns 128 b .. 128 b + 127, has the
-// scale 2^e, e the smallest exponent >= -126 with max|x| <= 448 * 2^e, and q = x 2^-e rounded to nearest even: |x - q 2^e| <= 2^-4 |x| down to e4m3's
-// subnormals (2^-10 of the scale).  A power of two because the matrix instruction of this chip (v_mfma_scale_f32_*_f8f6f4) multiplies by an e8m0 scale
+// Operand form: row m of a matrix [M][K] is Kp = K rounded up to 128 values of e4m3 (zero past K), laid out in slabs of 64: byte k of row m lies at
+// ((k / 64) * R + m) * 64 + k % 64, R = M rounded up to even (the row it adds is zero).  A tile's rows of one slab are one contiguous piece of memory,
+// read in whole cache lines; rows Kp apart give half lines (7936 x 4096 x 25088, 16-bit output: 668 us in slabs, 714 in rows; 8192^3: 402 and 432).
+// Block b of a row, columns 128 b .. 128 b + 127, has the scale 2^e, e the smallest exponent >= -126 with max|x| <= 448 * 2^e, and q = x 2^-e rounded
+// to nearest even: |x - q 2^e| <= 2^-4 |x| down to e4m3's subnormals (2^-10 of the scale).  A power of two because the matrix instruction of this chip (v_mfma_scale_f32_*_f8f6f4) multiplies by an e8m0 scale
 // per row and 32 columns itself: dividing by it rounds nothing and applying it costs nothing.  Non-finite elements become NaN and do not
 // enter the maximum: the products they take part in are NaN, the rest of the block keeps its scale.
 // Scales are bytes (e + 127), 128 rows to a group: byte ((b * G + m / 128) * 32 + m % 32) * 4 + (m / 32) % 4 with G = ceil(M / 128) -- one dword
@@ -14,6 +16,7 @@ namespace {
 
 constexpr int QB = 128;             // columns of a block
 
+__host__ __device__ __forceinline__ long slab_rows(long rows) { return (rows + 1) & ~1L; }
 __host__ __device__ __forceinline__ long scale_bytes(long rows, long blocks) { return blocks * ((rows + 127) / 128) * 128; }
 __device__ __forceinline__ long scale_at(long m, long blk, long groups) { return ((blk * groups + (m >> 7)) * 32 + (m & 31)) * 4 + ((m >> 5) & 3); }
 
@@ -67,7 +70,7 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(const T* __restrict__
     const int tk = (int)(blockIdx.x - tm * tilesK);
     const long m0 = tm * 128;
     const int k0 = tk * QB;
-    const long Kp = ((long)K + 127) / 128 * 128;
+    const long RM = slab_rows(M);
     float v[8][8];
     const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ldx * (long)sizeof(T)) % 16 == 0 && k0 + tc * 8 + 8 <= K;
     const T* p0 = x + (m0 + tr * 8) * ldx + k0 + tc * 8;
@@ -97,7 +100,7 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(const T* __restrict__
             }
             const int byte = scale_byte(top);
             const long m = m0 + tr * 8 + i;
-            if (m < M) *reinterpret_cast<u32x2*>(rows + m * Kp + k0 + tc * 8) = pack_fp8x8(v[i], scale_inv(byte), inf);
+            if (m < RM) *reinterpret_cast<u32x2*>(rows + ((2L * tk + (tc >> 3)) * RM + m) * 64 + (tc & 7) * 8) = pack_fp8x8(v[i], scale_inv(byte), inf);
             if (tc == 0) rbyte[tr * 8 + i] = (unsigned char)byte;                        // (rows past M of the last group: blocks of zeros)
         }
     }
@@ -118,7 +121,7 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(const T* __restrict__
                 rbyte[tid] | (unsigned)rbyte[tid + 32] << 8 | (unsigned)rbyte[tid + 64] << 16 | (unsigned)rbyte[tid + 96] << 24;
         }
     if constexpr (COLS) {
-        const long Mp = (M + 127) / 128 * 128, groups = ((long)K + 127) / 128;
+        const long RK = slab_rows(K), groups = ((long)K + 127) / 128;
         if (tid < 128) {
             float top = 0.f;
 #pragma unroll
@@ -163,7 +166,7 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(const T* __restrict__
             const int c = p * 32 + (tid >> 3), h = tid & 7, key = c >> 3;               // 16 bytes: pieces 2h and 2h + 1
             const u32x2 a = *reinterpret_cast<const u32x2*>(tile + c * 128 + (((2 * h) ^ key) << 3));
             const u32x2 b = *reinterpret_cast<const u32x2*>(tile + c * 128 + (((2 * h + 1) ^ key) << 3));
-            if (k0 + c < K) *reinterpret_cast<u32x4*>(cols + (long)(k0 + c) * Mp + m0 + h * 16) = u32x4{a.x, a.y, b.x, b.y};
+            if (k0 + c < RK) *reinterpret_cast<u32x4*>(cols + ((2 * tm + (h >> 2)) * RK + k0 + c) * 64 + (h & 3) * 16) = u32x4{a.x, a.y, b.x, b.y};
         }
         if constexpr (SUM)
             if (tid < 128 && k0 + tid < K) {                      // this tile's 128 rows; the tiles' sums are added in order by the caller
@@ -343,17 +346,18 @@ __global__ __launch_bounds__(256) void fp8_few_rows_kernel(const Fp8Args g, floa
     const long n0 = (long)(blockIdx.x / slices) * 32;
     const int blocks = (int)(g.Kp / 128), b0 = min(slice * per, blocks), b1 = min(b0 + per, blocks);
     const long gA = ((long)g.M + 127) / 128, gW = ((long)g.N + 127) / 128;
-    const unsigned char* wp = g.W + min(n0 + fr, (long)g.N - 1) * g.Kp + fh * 16;
-    const unsigned char* ap = g.A + (long)min(fr, g.M - 1) * g.Kp + fh * 16;
+    const long RA = slab_rows(g.M) * 64, RW = slab_rows(g.N) * 64;
+    const unsigned char* wp = g.W + min(n0 + fr, (long)g.N - 1) * 64 + fh * 16;
+    const unsigned char* ap = g.A + (long)min(fr, g.M - 1) * 64 + fh * 16;
     const unsigned* sw = reinterpret_cast<const unsigned*>(g.Ws) + (n0 >> 7) * 32 + fr;
     const unsigned* sa = reinterpret_cast<const unsigned*>(g.As) + fr;
     const int shift = (int)(n0 >> 5 & 3) * 8;
     struct { u32x4 w[4], a[4]; unsigned ew, ea; } buf[DEPTH];
     auto fetch = [&](auto& t, int b) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) t.w[c] = *reinterpret_cast<const u32x4*>(wp + (long)b * 128 + c * 32);
+        for (int c = 0; c < 4; ++c) t.w[c] = *reinterpret_cast<const u32x4*>(wp + (2L * b + (c >> 1)) * RW + (c & 1) * 32);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) t.a[c] = *reinterpret_cast<const u32x4*>(ap + (long)b * 128 + c * 32);
+        for (int c = 0; c < 4; ++c) t.a[c] = *reinterpret_cast<const u32x4*>(ap + (2L * b + (c >> 1)) * RA + (c & 1) * 32);
         t.ew = sw[(long)b * gW * 32];
         t.ea = sa[(long)b * gA * 32];
     };
@@ -402,8 +406,9 @@ __global__ __launch_bounds__(1024) void fp8_few16_kernel(const Fp8Args g, float*
     const int blocks = (int)(g.Kp / 128), b0 = min(slice * per, blocks), b1 = min(b0 + per, blocks);
     const long gA = ((long)g.M + 127) / 128, gW = ((long)g.N + 127) / 128;
     const long n = min(n0 + fr, (long)g.N - 1);
-    const unsigned char* wp = g.W + n * g.Kp + fq * 16;
-    const unsigned char* ap = g.A + (long)min(fr, g.M - 1) * g.Kp + fq * 16;
+    const long RA = slab_rows(g.M) * 64, RW = slab_rows(g.N) * 64;
+    const unsigned char* wp = g.W + n * 64 + fq * 16;
+    const unsigned char* ap = g.A + (long)min(fr, g.M - 1) * 64 + fq * 16;
     const unsigned* sw = reinterpret_cast<const unsigned*>(g.Ws) + (n >> 7) * 32 + (n & 31);
     const unsigned* sa = reinterpret_cast<const unsigned*>(g.As) + fr;
     const int shift = (int)(n >> 5 & 3) * 8;
@@ -411,8 +416,8 @@ __global__ __launch_bounds__(1024) void fp8_few16_kernel(const Fp8Args g, float*
     auto fetch = [&](auto& t, int b) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            t.w[c] = *reinterpret_cast<const u32x4*>(wp + (long)b * 128 + c * 64);
-            t.a[c] = *reinterpret_cast<const u32x4*>(ap + (long)b * 128 + c * 64);
+            t.w[c] = *reinterpret_cast<const u32x4*>(wp + (2L * b + c) * RW);
+            t.a[c] = *reinterpret_cast<const u32x4*>(ap + (2L * b + c) * RA);
         }
         t.ew = sw[(long)b * gW * 32];
         t.ea = sa[(long)b * gA * 32];
@@ -465,13 +470,14 @@ __global__ __launch_bounds__(512) void fp8_tile_kernel(const Fp8Args g, float* _
     const long gA = ((long)g.M + 127) / 128, gW = ((long)g.N + 127) / 128;
     const unsigned *sa = reinterpret_cast<const unsigned*>(g.As) + (long)tm * 32 + fr, *sw = reinterpret_cast<const unsigned*>(g.Ws) + (long)tn * 32 + fr;
     // thread -> rows tid / 8 + 32 p, 16-byte piece tid % 8, stored at the piece permuted by half the row number (16 rows' reads of one piece then hit every bank once)
+    const long RA = slab_rows(g.M), RW = slab_rows(g.N);
     const unsigned char *ap[4], *wp[4];
     int at[4];
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
         const int r = p * 32 + (tid >> 3), h = tid & 7;
-        ap[p] = g.A + min(m0 + r, (long)g.M - 1) * g.Kp + h * 16;
-        wp[p] = g.W + min(n0 + r, (long)g.N - 1) * g.Kp + h * 16;
+        ap[p] = g.A + ((h >> 2) * RA + min(m0 + r, (long)g.M - 1)) * 64 + (h & 3) * 16;
+        wp[p] = g.W + ((h >> 2) * RW + min(n0 + r, (long)g.N - 1)) * 64 + (h & 3) * 16;
         at[p] = r * 128 + ((h ^ (r >> 1 & 7)) << 4);
     }
     u32x4 ra[4], rw[4];
@@ -479,8 +485,8 @@ __global__ __launch_bounds__(512) void fp8_tile_kernel(const Fp8Args g, float* _
     auto fetch = [&](int b) {
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
-            ra[p] = *reinterpret_cast<const u32x4*>(ap[p] + (long)b * 128);
-            rw[p] = *reinterpret_cast<const u32x4*>(wp[p] + (long)b * 128);
+            ra[p] = *reinterpret_cast<const u32x4*>(ap[p] + b * RA * 128);
+            rw[p] = *reinterpret_cast<const u32x4*>(wp[p] + b * RW * 128);
         }
         ea_n = sa[(long)b * gA * 32];
         ew_n = sw[(long)b * gW * 32];
@@ -594,17 +600,17 @@ __global__ __launch_bounds__(512) void fp8_pingpong_kernel(const Fp8Args g, floa
     // ---- loads to LDS: a slab is (16 + 8 NI) pieces of 16 rows, the rows of A, then those of W; wave w loads pieces PIECES w + j.  Global address = the
     // piece's uniform base + a lane offset that never changes + the instruction's immediate, which also moves the LDS address: piece j lands j KiB
     // behind ONE LDS base (the lane offset carries -j KiB, and 3 KiB that the uniform base gives back keep it unsigned)
-    const char *base_a = reinterpret_cast<const char*>(g.A + m0 * g.Kp) - 3072, *base_w = reinterpret_cast<const char*>(g.W + n0 * g.Kp) - 3072;
+    const char *base_a = reinterpret_cast<const char*>(g.A + m0 * 64) - 3 * 1024, *base_w = reinterpret_cast<const char*>(g.W + n0 * 64) - 3 * 1024;
+    const long step_a = slab_rows(g.M) * 64, step_w = slab_rows(g.N) * 64;              // from slab to slab
     unsigned vo[4] = {};
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
         const int r = (PIECES * wave + j) * 16 + (lane >> 2);
         const long row = r < 256 ? min(m0 + r, (long)g.M - 1) - m0 : min(n0 + r - 256, (long)g.N - 1) - n0;        // (rows past the end: the last one again)
-        vo[j] = (unsigned)(row * g.Kp) + ((lane & 3) ^ ((r >> 2) & 3)) * 16 + 3072u - 1024u * j;
+        vo[j] = (unsigned)(row * 64) + ((lane & 3) ^ ((r >> 2) & 3)) * 16 + 1024u * (3 - j);
     }
     unsigned vo_0 = vo[0], vo_1 = vo[1], vo_2 = vo[2], vo_3 = vo[3];
-    const char *const base_0 = PIECES * wave < 16 ? base_a : base_w, *const base_1 = PIECES * wave + 1 < 16 ? base_a : base_w,
-               *const base_2 = PIECES * wave + 2 < 16 ? base_a : base_w, *const base_3 = PIECES * wave + 3 < 16 ? base_a : base_w;
+    const bool a_0 = PIECES * wave < 16, a_1 = PIECES * wave + 1 < 16, a_2 = PIECES * wave + 2 < 16, a_3 = PIECES * wave + 3 < 16;
     const int lds_rows0 = PIECES * wave * 16 * PP_ROW;
     const long gA = ((long)g.M + 127) / 128, gW = ((long)g.N + 127) / 128;
     const unsigned* sp = lane < 32 ? reinterpret_cast<const unsigned*>(g.As) + ((long)b0 * gA + min((long)tm * 2 + grp, gA - 1)) * 32 + fr
@@ -617,15 +623,15 @@ __global__ __launch_bounds__(512) void fp8_pingpong_kernel(const Fp8Args g, floa
         __builtin_amdgcn_global_load_lds((glb_void_t*)sp, (lds_void_t*)(sreg + ((kt >> 1) & 3) * 2048), 4, 0, 0);
         if (++sblock < b1) sp += sstep;
     };
-    auto slab_off = [&](int kt) { return (long)min(kt, nt - 1) * PP_ROW; };
     auto issue = [&](int kt) {
-        const long k = slab_off(kt);
-        char* dst = smem + (kt & (D - 1)) * PP_STAGE + lds_rows0;
+        const long k = min(kt, nt - 1);
+        const char *sa = base_a + k * step_a, *sw = base_w + k * step_w;
+        char* to = smem + (kt & (D - 1)) * PP_STAGE + lds_rows0;
         if (!(kt & 1)) issue_scales(kt);
-        lds_piece<0>(uniform_ptr(base_0 + k), vo_0, dst);
-        lds_piece<1024>(uniform_ptr(base_1 + k), vo_1, dst);
-        lds_piece<2048>(uniform_ptr(base_2 + k), vo_2, dst);
-        if constexpr (NI == 2) lds_piece<3072>(uniform_ptr(base_3 + k), vo_3, dst);
+        lds_piece<0>(uniform_ptr(a_0 ? sa : sw), vo_0, to);
+        lds_piece<1024>(uniform_ptr(a_1 ? sa : sw), vo_1, to);
+        lds_piece<2048>(uniform_ptr(a_2 ? sa : sw), vo_2, to);
+        if constexpr (NI == 2) lds_piece<3 * 1024>(uniform_ptr(a_3 ? sa : sw), vo_3, to);
     };
 
     // LDS byte addresses of the lane's pieces fh and fh + 2 in slab 0: its first row of A and of W (the others 32 rows = 2 KiB further, same permutation)
@@ -644,8 +650,9 @@ __global__ __launch_bounds__(512) void fp8_pingpong_kernel(const Fp8Args g, floa
         const unsigned st = (kt & (D - 1)) * PP_STAGE;
         ra0 = at_a + st, ra1 = ra0 ^ 32, rw0 = at_w + st, rw1 = rw0 ^ 32;
         rs = at_s + ((kt >> 1) & 3) * 2048;
-        const long k = slab_off(kt + D - 1);
-        u0 = uniform_ptr(base_0 + k), u1 = uniform_ptr(base_1 + k), u2 = uniform_ptr(base_2 + k), u3 = uniform_ptr(base_3 + k);
+        const long k = min(kt + D - 1, nt - 1);
+        const char *sa = base_a + k * step_a, *sw = base_w + k * step_w;
+        u0 = uniform_ptr(a_0 ? sa : sw), u1 = uniform_ptr(a_1 ? sa : sw), u2 = uniform_ptr(a_2 ? sa : sw), u3 = uniform_ptr(a_3 ? sa : sw);
         dst = ((kt + D - 1) & (D - 1)) * PP_STAGE + lds_rows0;
     };
     auto load_frags = [&](bool even) {
@@ -719,7 +726,7 @@ __global__ __launch_bounds__(512) void fp8_pingpong_kernel(const Fp8Args g, floa
         lds_piece<2048>(u2, vo_2, to);
         __builtin_amdgcn_sched_barrier(0);
         FP8_MMA(3)
-        if constexpr (NI == 2) lds_piece<3072>(u3, vo_3, to);
+        if constexpr (NI == 2) lds_piece<3 * 1024>(u3, vo_3, to);
         __builtin_amdgcn_s_setprio(0);
         __builtin_amdgcn_sched_barrier(0);
         prepare(kt + 1);
@@ -796,11 +803,10 @@ Fp8Plan fp8_plan(int64_t M, int64_t N, int64_t Kp) {
         want = min(256 / max(tiles, one), blocks / (M <= 16 ? 32 : 64));
     } else {
         const int64_t c128 = (t128 + 255) / 256 * 27, chalf = (thalf + 255) / 256 * 41, cfull = (tfull + 255) / 256 * 51;
-        const bool big = blocks >= 1 && Kp <= (1 << 23);                      // (32-bit lane offsets inside a tile's 256 rows)
-        if (big && cfull <= c128 && cfull <= chalf) {
+        if (blocks >= 1 && cfull <= c128 && cfull <= chalf) {
             kernel = FP8_FULL;
             tiles = tfull;
-        } else if (big && chalf <= c128) {
+        } else if (blocks >= 1 && chalf <= c128) {
             kernel = FP8_HALF;
             tiles = thalf;
         } else {

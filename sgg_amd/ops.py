@@ -1260,16 +1260,20 @@ def layer_norm_bwd(dy, x, mean, rstd, weight=None, want_dx=True, want_dw=True, w
 
 
 class Fp8Rows(object):
-    """A matrix [M, K] in the 8-bit operand form of include/sgg_hip.h: `data` float8_e4m3fn [M, K rounded up to 128], `scale` the exponent
-    bytes of its blocks of 128 columns (the kernels' order), `shape` = (M, K)."""
+    """A matrix [M, K] in the 8-bit operand form of include/sgg_hip.h: `data` float8_e4m3fn [slabs of 64 columns, M rounded up to even, 64],
+    `scale` the exponent bytes of its blocks of 128 columns (the kernels' order), `shape` = (M, K)."""
     __slots__ = ('data', 'scale', 'shape')
 
     def __init__(self, data, scale, shape):
         self.data, self.scale, self.shape = data, scale, tuple(shape)
 
+    def codes(self):
+        """-> float8_e4m3fn [M, K rounded up to 128], the rows as rows"""
+        return self.data[:, :self.shape[0]].transpose(0, 1).reshape(self.shape[0], -1)
+
     def exponents(self):
         """-> int32 [M, blocks]: block b of row m stands for its e4m3 values times 2^exponents[m, b]"""
-        M, blocks = self.shape[0], self.data.shape[1] // FP8_BLOCK
+        M, blocks = self.shape[0], self.data.shape[0] // 2
         e = self.scale.view(blocks, -1, 32, 4).permute(1, 3, 2, 0).reshape(-1, blocks)        # (block, group, r % 32, r / 32) -> rows
         return e[:M].int() - 127
 
@@ -1277,13 +1281,18 @@ class Fp8Rows(object):
         """-> f64 [M, K], the values the operand stands for, each of them exact (fp32's largest rounds to 2^128, which fp32 has not)"""
         M, K = self.shape
         e = ((self.exponents().long() + 1023) << 52).view(torch.float64)                      # 2^e itself
-        return (self.data.float().double().view(M, -1, FP8_BLOCK) * e[:, :, None]).reshape(M, self.data.shape[1])[:, :K]
+        return (self.codes().float().double().view(M, -1, FP8_BLOCK) * e[:, :, None]).reshape(M, -1)[:, :K]
+
+
+def _fp8_dims(M, K):
+    """slabs, rows of a slab, scales"""
+    blocks = (K + FP8_BLOCK - 1) // FP8_BLOCK
+    return 2 * blocks, (M + 1) & ~1, (M + 127) // 128 * 128 * blocks         # (the last: sgg_fp8_scale_bytes)
 
 
 def _fp8_empty(M, K, device):
-    Kp = (K + FP8_BLOCK - 1) // FP8_BLOCK * FP8_BLOCK
-    return Fp8Rows(torch.empty((M, Kp), dtype=torch.float8_e4m3fn, device=device),
-                   torch.empty((M + 127) // 128 * Kp, dtype=torch.uint8, device=device), (M, K))        # sgg_fp8_scale_bytes(M, K)
+    slabs, R, scales = _fp8_dims(M, K)
+    return Fp8Rows(torch.empty((slabs, R, 64), dtype=torch.float8_e4m3fn, device=device), torch.empty(scales, dtype=torch.uint8, device=device), (M, K))
 
 
 def quantize_fp8(x, form='rows', colsum=False):
@@ -1320,8 +1329,8 @@ def gemm_fp8(A, W, bias=None, act=ACT_NONE, out_dtype=torch.float32, out=None):
         d, sc, (rows, cols) = q.data, q.scale, q.shape
         _here(d, 'gemm_fp8')
         _here(sc, 'gemm_fp8')
-        Kp = (cols + FP8_BLOCK - 1) // FP8_BLOCK * FP8_BLOCK
-        if d.dtype != torch.float8_e4m3fn or sc.dtype != torch.uint8 or d.shape != (rows, Kp) or sc.numel() != (rows + 127) // 128 * Kp:
+        slabs, R, scales = _fp8_dims(rows, cols)
+        if d.dtype != torch.float8_e4m3fn or sc.dtype != torch.uint8 or d.shape != (slabs, R, 64) or sc.numel() != scales:
             raise ValueError('sgg_amd: gemm_fp8: operand [%d, %d] holds %s %s and %d scales' % (rows, cols, d.dtype, tuple(d.shape), sc.numel()))
     b = _vector(bias, N, 'gemm_fp8 bias')
     if out is None:
@@ -1331,6 +1340,7 @@ def gemm_fp8(A, W, bias=None, act=ACT_NONE, out_dtype=torch.float32, out=None):
         if tuple(out.shape) != (M, N):
             raise ValueError('sgg_amd: gemm_fp8: out %s for a [%d, %d] product' % (tuple(out.shape), M, N))
     ldc, code = _row_matrix(out, 'gemm_fp8 out'), dt(out)
+    Kp = slabs * 64
     splits = _lib.load().sgg_gemm_fp8_splits(M, N, Kp)
     _lib.check(min(splits, 0), 'sgg_gemm_fp8_splits')
     ws = _ws(splits * M * N, out.device) if splits > 1 else None

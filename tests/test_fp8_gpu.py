@@ -52,12 +52,12 @@ def test_operand_form_is_the_definition(M, K, dtype):
     from sgg_amd import ops
     x = rand(M, K, dtype, M + K)
     r, c = ops.quantize_fp8(x, 'both')
-    assert r.shape == (M, K) and c.shape == (K, M) and r.data.shape == (M, (K + 127) // 128 * 128)
+    assert r.shape == (M, K) and c.shape == (K, M) and r.data.shape == ((K + 127) // 128 * 2, M + M % 2, 64)
     for q, src in ((r, x), (c, x.t().contiguous())):
         v, e = grid(src)
         assert torch.equal(q.exponents(), e.int())
         same(q.dequantize(), v)
-        assert not q.data.view(torch.uint8)[:, q.shape[1]:].any()                         # zeros past the last column
+        assert not q.codes().view(torch.uint8)[:, q.shape[1]:].any() and not q.data.view(torch.uint8)[:, q.shape[0]:].any()     # zeros past the last column and row
     alone, alone_t = ops.quantize_fp8(x), ops.quantize_fp8(x, 'cols')
     assert torch.equal(alone.data.view(torch.uint8), r.data.view(torch.uint8)) and torch.equal(alone.scale, r.scale)
     assert torch.equal(alone_t.data.view(torch.uint8), c.data.view(torch.uint8)) and torch.equal(alone_t.scale, c.scale)
@@ -385,7 +385,7 @@ def test_refusals():
         ops.gemm_fp8(x, A)
     with pytest.raises(ValueError):
         ops.gemm_fp8(A, ops.quantize_fp8(x[:, :255]))                     # same padded width, another reduction
-    for bad in (ops.Fp8Rows(A.data[:3], A.scale, (4, 256)), ops.Fp8Rows(A.data, A.scale[:100], (4, 256)), ops.Fp8Rows(A.data, A.scale, (4, 300)),
+    for bad in (ops.Fp8Rows(A.data[:3], A.scale, (4, 256)), ops.Fp8Rows(A.data, A.scale[:100], (4, 256)), ops.Fp8Rows(A.data, A.scale, (4, 300)), ops.Fp8Rows(A.codes(), A.scale, (4, 256)),
                 ops.Fp8Rows(A.data.view(torch.uint8), A.scale, (4, 256))):
         with pytest.raises(ValueError):                                   # an operand whose memory is not its shape's
             ops.gemm_fp8(bad, bad)

@@ -90,7 +90,8 @@ def test_cpu_tensors_are_refused():
 
 
 def test_operand_form_index_rule():
-    """byte ((b G + m / 128) 32 + m % 32) 4 + (m / 32) % 4 holds the exponent of row m, block b; values are e4m3 times 2^e"""
+    """byte ((b G + m / 128) 32 + m % 32) 4 + (m / 32) % 4 holds the exponent of row m, block b; byte ((k / 64) R + m) 64 + k % 64 the code of row m,
+    column k; values are e4m3 times 2^e"""
     from sgg_amd import ops
     M, K = 300, 200
     G, blocks = 3, 2
@@ -101,7 +102,11 @@ def test_operand_form_index_rule():
         for b in range(blocks):
             scale[((b * G + m // 128) * 32 + m % 32) * 4 + m // 32 % 4] = int(e[m, b]) + 127
     data = torch.randint(0, 127, (M, 256), dtype=torch.uint8, generator=gen).view(torch.float8_e4m3fn)
-    q = ops.Fp8Rows(data, scale, (M, K))
+    slabs = torch.zeros(4 * 300 * 64, dtype=torch.uint8)
+    for k in range(256):
+        slabs[(k // 64 * 300 + torch.arange(M)) * 64 + k % 64] = data.view(torch.uint8)[:, k]
+    q = ops.Fp8Rows(slabs.view(torch.float8_e4m3fn).view(4, 300, 64), scale, (M, K))
+    assert torch.equal(q.codes().view(torch.uint8), data.view(torch.uint8))
     assert torch.equal(q.exponents(), e.int())
     want = data.double() * (2.0 ** e.double()).repeat_interleave(128, 1)
     assert q.dequantize().shape == (M, K) and torch.equal(q.dequantize().double(), want[:, :K])
