@@ -22,7 +22,7 @@
 extern "C" {
 #endif
 
-#define SGG_ABI_VERSION 17   /* bump whenever a prototype below changes: tests/abi.lock pins (version, digest of the prototypes) */
+#define SGG_ABI_VERSION 18   /* bump whenever a prototype below changes: tests/abi.lock pins (version, digest of the prototypes) */
 
 enum { SGG_F32 = 0, SGG_BF16 = 1, SGG_F16 = 2,
        /* a PAIR of f16 planes x = hi + lo (hi = f16(x), lo = f16(x - hi): 22 significand bits) -- the operand / activation format of the x3
@@ -424,11 +424,11 @@ int sgg_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ldx
  * colsum f32[K] (or NULL; only with `cols`): the column sums of x (a bias gradient of x = dY), added in a fixed order; colsum_ws
  * f32[ceil(M / 128) * K] then.
  * gemm_fp8: C[m][n] = act(sum_k A[m][k] W[n][k] + bias[n]), fp32 accumulation, one rounding to out_dtype; bias f32[N] or NULL; ldc in
- * elements; ws f32[splits * M * N] when sgg_gemm_fp8_splits(M, N, Kp) is more than 1 (the K slices are added in a fixed order). */
+ * elements; ws f32[splits * M * N] when sgg_gemm_fp8_splits(M, N, Kp, out_dtype) is more than 1 (the K slices are added in a fixed order). */
 int64_t sgg_fp8_scale_bytes(int64_t rows, int64_t K);
 int sgg_fp8_quantize(const void* x, int64_t ldx, int64_t M, int64_t K, void* rows, void* rows_scale, void* cols, void* cols_scale, float* colsum,
                      float* colsum_ws, int dtype, void* stream);
-int sgg_gemm_fp8_splits(int64_t M, int64_t N, int64_t Kp);
+int sgg_gemm_fp8_splits(int64_t M, int64_t N, int64_t Kp, int out_dtype);
 int sgg_gemm_fp8(const void* A, const void* A_scale, const void* W, const void* W_scale, const float* bias, void* C, int64_t ldc, int64_t M, int64_t N,
                  int64_t Kp, int act, int out_dtype, float* ws, void* stream);
 

@@ -12,7 +12,7 @@ LIB_PATH = os.environ.get('SGG_HIP_LIB') or os.path.join(_HERE, 'libsgg_hip.so')
 
 SGG_F32, SGG_BF16, SGG_F16 = 0, 1, 2
 ACT_NONE, ACT_RELU = 0, 1
-ABI_VERSION = 17
+ABI_VERSION = 18
 
 import threading  # noqa: E402
 # held by sgg_amd.graph_step while it captures a hipGraph, and by every other thread of this package around its own GPU calls (the
@@ -119,7 +119,7 @@ SIGNATURES = {
     'sgg_layer_norm_bwd': [_P, _L, _P, _L, _P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _P],
     'sgg_fp8_scale_bytes': [_L, _L],
     'sgg_fp8_quantize': [_P, _L, _L, _L, _P, _P, _P, _P, _P, _P, _I, _P],
-    'sgg_gemm_fp8_splits': [_L, _L, _L],
+    'sgg_gemm_fp8_splits': [_L, _L, _L, _I],
     'sgg_gemm_fp8': [_P, _P, _P, _P, _P, _P, _L, _L, _L, _L, _I, _I, _P, _P],
     'sgg_clip_grads_parts': [_I],
     'sgg_clip_grads': [_P, _P, _P, _P, _P, _I, _D, _D, _P, _P, _P],

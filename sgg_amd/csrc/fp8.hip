@@ -788,35 +788,36 @@ enum { FP8_FEW16, FP8_FEW, FP8_TILE, FP8_HALF, FP8_FULL };
 struct Fp8Plan { int kernel, tiles, slices, per; };
 
 // Few rows: the stream kernels; W in slices only where its rows alone leave CUs idle and every wave keeps two blocks or more.
-// Otherwise the cheapest of the three tilings by rounds of the 256 CUs, in us per round measured at K = 4096 (16-bit outputs): 128 x 128 tiles 27, 256 x 128 tiles
-// 41, 256 x 256 tiles 51.  E.g. 1024 x 4096: 27 / 41 / 51 -> 128 x 128 (measured 27.6 / 32.7 / 39.6 us); 4096 x 2048: 54 / 41 / 51 -> 256 x 128 (50.1 / 40.5 /
-// 50.5); 3000 x 3000 (K = 1000): 81 / 82 / 51 -> 256 x 256 (25.1 / 26.8 / 22.0 us).
-// 128 x 128 tiles that leave CUs idle are cut along K, 16 blocks or more to a slice, in two only from 48 blocks on (a join launch costs what some 8 steps do:
-// 512 x 4096 x 4096 takes 25.2 us whole, 27.2 in two slices; 256 x 4096 x 25088 43.9 in four).
-Fp8Plan fp8_plan(int64_t M, int64_t N, int64_t Kp) {
+// Otherwise the cheapest of the three tilings and of its cuts along K: rounds of the 256 CUs x blocks of a slice x ns per block (STEP), and for a cut the
+// join: its launch, its partial outputs written and read at 5 TB/s, half a us per slice.  Measured (us; 16-bit | fp32 outputs):
+//                        128 x 128          256 x 128          256 x 256        chosen
+//   1024 x 4096 x 4096   28.2 | 40.9        29.6 | 47.6 (2)    39.6 | 53.0 (3)  128 x 128
+//   4096 x 2048 x 4096   55.0 | 84.0        36.0 | 64.5        50.4 | 77.1 (2)  256 x 128
+//   512 x 4608 x 7936    45.1 | 61.9        33.5 | 50.3 (3)    40.1 | 54.7 (4)  256 x 128 in 3 slices
+//   256 x 4096 x 25088   46.5 | 64.7 (4)    41.8 | 60.7 (8)    45.7 | 65.4 (12) 256 x 128 in 8 slices
+//   256 x 1024 x 7936    18.5 | 21.5 (8)    19.3 | 24.6 (8)    24.3 | 31.2 (8)  128 x 128 in 8 slices
+//   128 x 512 x 4096     13.3 | 14.4 (8)    13.2 | 15.8 (8)    16.4 | 19.0 (8)  128 x 128 in 8 slices (one slice: 24.5 | 35.0)
+//   4096 x 4096 x 7936   -                  -                  101 | 186        256 x 256
+// (slices in brackets)
+Fp8Plan fp8_plan(int64_t M, int64_t N, int64_t Kp, bool wide) {
     const int64_t blocks = Kp / 128, one = 1;
-    const int64_t t128 = ((M + 127) / 128) * ((N + 127) / 128), thalf = ((M + 255) / 256) * ((N + 127) / 128), tfull = ((M + 255) / 256) * ((N + 255) / 256);
-    int64_t kernel, tiles, want = 1;
+    int64_t kernel = FP8_TILE, tiles, slices = 1;
     if (M <= 32) {
         kernel = M <= 16 ? FP8_FEW16 : FP8_FEW;
         tiles = M <= 16 ? (N + 15) / 16 : (N + 31) / 32;
-        want = min(256 / max(tiles, one), blocks / (M <= 16 ? 32 : 64));
+        slices = max(min(256 / max(tiles, one), blocks / (M <= 16 ? 32 : 64)), one);
     } else {
-        const int64_t c128 = (t128 + 255) / 256 * 27, chalf = (thalf + 255) / 256 * 41, cfull = (tfull + 255) / 256 * 51;
-        if (blocks >= 1 && cfull <= c128 && cfull <= chalf) {
-            kernel = FP8_FULL;
-            tiles = tfull;
-        } else if (blocks >= 1 && chalf <= c128) {
-            kernel = FP8_HALF;
-            tiles = thalf;
-        } else {
-            kernel = FP8_TILE;
-            tiles = t128;
-            want = min(256 / max(tiles, one), blocks / 16);
-            if (want == 2 && blocks < 48) want = 1;
-        }
+        static const int64_t STEP[2][3] = {{700, 1000, 1500}, {1000, 1600, 2900}}, JOIN = 4000;
+        const int64_t count[3] = {((M + 127) / 128) * ((N + 127) / 128), ((M + 255) / 256) * ((N + 127) / 128), ((M + 255) / 256) * ((N + 255) / 256)};
+        tiles = count[0];
+        double best = -1;
+        for (int k = 0; k < 3 && blocks; ++k)
+            for (int64_t s = 1; s == 1 || (s * count[k] <= 256 && s <= min(blocks / 2, (int64_t)32)); ++s) {
+                const double t = (double)((count[k] * s + 255) / 256 * ((blocks + s - 1) / s) * STEP[wide][k]) + (s > 1 ? JOIN + 500 * s + (double)s * M * N / 625 : 0.);
+                if (best < 0 || t < best) best = t, kernel = FP8_TILE + k, tiles = count[k], slices = s;
+            }
     }
-    const int64_t slices = max(want, one), per = max((blocks + slices - 1) / slices, one);
+    const int64_t per = max((blocks + slices - 1) / slices, one);
     return {(int)kernel, tiles * slices > 0x7fffffff ? -1 : (int)tiles, (int)max((blocks + per - 1) / per, one), (int)per};       // (no empty slice)
 }
 
@@ -865,9 +866,10 @@ extern "C" int sgg_fp8_quantize(const void* x, int64_t ldx, int64_t M, int64_t K
 }
 
 // K slices of a product whose output tiles alone do not fill the chip; ws then holds that many fp32 [M][N] partial outputs
-extern "C" int sgg_gemm_fp8_splits(int64_t M, int64_t N, int64_t Kp) {
+extern "C" int sgg_gemm_fp8_splits(int64_t M, int64_t N, int64_t Kp, int out_dtype) {
+    if (!sgg_is_dtype(out_dtype)) return SGG_ERR_DTYPE;
     if (M < 0 || N < 0 || Kp < 0 || Kp % 128 || M > 0x7fffff00 || N > 0x7fffff00 || Kp > 0x7fffff00) return SGG_ERR_ARG;
-    return fp8_plan(M, N, Kp).slices;
+    return fp8_plan(M, N, Kp, out_dtype == SGG_F32).slices;
 }
 
 extern "C" int sgg_gemm_fp8(const void* A, const void* A_scale, const void* W, const void* W_scale, const float* bias, void* C, int64_t ldc, int64_t M,
@@ -877,7 +879,7 @@ extern "C" int sgg_gemm_fp8(const void* A, const void* A_scale, const void* W, c
         return SGG_ERR_ARG;
     if (M == 0 || N == 0) return SGG_OK;
     if (!C || (Kp > 0 && (!A || !A_scale || !W || !W_scale)) || (((uintptr_t)A | (uintptr_t)W) & 15) || (((uintptr_t)A_scale | (uintptr_t)W_scale) & 3)) return SGG_ERR_ARG;
-    const Fp8Plan p = fp8_plan(M, N, Kp);
+    const Fp8Plan p = fp8_plan(M, N, Kp, out_dtype == SGG_F32);
     if (p.tiles < 0 || (p.slices > 1 && !ws)) return SGG_ERR_ARG;
     const Fp8Args g = {(const unsigned char*)A, (const unsigned char*)A_scale, (const unsigned char*)W, (const unsigned char*)W_scale, bias, (char*)C, (long)ldc, (long)Kp, (int)M, (int)N, act, out_dtype};
     hipStream_t s = (hipStream_t)stream;

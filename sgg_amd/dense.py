@@ -177,6 +177,8 @@ def affine_fp8(x, weight, bias=None, out_dtype=None):
     """x [..., K] (f32 / bf16 / f16) -> [..., N] = x . weight^T + bias in 8-bit floating point (ops.gemm_fp8), out_dtype (default x's type);
     differentiable in all three, the gradients' products in 8 bits too.  What set_compute('fp8') makes of affine / conv2d."""
     _need_gpu(x)
+    if x.dim() == 2:                                 # (no views in autograd's graph: ~10 us of the host's each way)
+        return _affine_fp8_rows(x, weight, bias, out_dtype or x.dtype)
     return _affine_fp8_rows(x.reshape(-1, x.shape[-1]), weight, bias, out_dtype or x.dtype).view(*x.shape[:-1], weight.shape[0])
 
 
@@ -346,10 +348,12 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Layer normalisation over the last axis of x [..., C] (f32 / bf16 / f16; statistics and sums in fp32) with weight, bias f32[C] or None
     -> x's shape and type; differentiable in all three (csrc/layernorm.hip: one pass each way)."""
     _need_gpu(x)
-    rows = x.reshape(-1, x.shape[-1])
-    if not (torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad))):
-        return ops._layer_norm(_row_form(rows), weight, bias, eps, False)[0].view(x.shape)
-    return _LayerNorm.apply(rows, weight, bias, eps).view(x.shape)
+    rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])           # (no views in autograd's graph where none are needed)
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
+        y = _LayerNorm.apply(rows, weight, bias, eps)
+    else:
+        y = ops._layer_norm(_row_form(rows), weight, bias, eps, False)[0]
+    return y if x.dim() == 2 else y.view(x.shape)
 
 
 class LayerNormRows(nn.LayerNorm):

@@ -1341,7 +1341,7 @@ def gemm_fp8(A, W, bias=None, act=ACT_NONE, out_dtype=torch.float32, out=None):
             raise ValueError('sgg_amd: gemm_fp8: out %s for a [%d, %d] product' % (tuple(out.shape), M, N))
     ldc, code = _row_matrix(out, 'gemm_fp8 out'), dt(out)
     Kp = slabs * 64
-    splits = _lib.load().sgg_gemm_fp8_splits(M, N, Kp)
+    splits = _lib.load().sgg_gemm_fp8_splits(M, N, Kp, code)
     _lib.check(min(splits, 0), 'sgg_gemm_fp8_splits')
     ws = _ws(splits * M * N, out.device) if splits > 1 else None
     _lib.call('sgg_gemm_fp8', _p(A.data), _p(A.scale), _p(W.data), _p(W.scale), b, out.data_ptr(), ldc, M, N, Kp, act, code, _p(ws), _stream())

@@ -50,10 +50,11 @@ def test_fp8_entries_refuse():
                 dict(act=2), dict(A=P + 8), dict(Ws=P + 1), dict(M=1 << 33)):
         assert g(**bad) == ERR_ARG, bad
     assert g(dtype=3) == ERR_DTYPE and g(M=0, A=None) == 0 and g(N=0, C=None) == 0
-    assert lib.sgg_gemm_fp8_splits(-1, 4, 128) == ERR_ARG and lib.sgg_gemm_fp8_splits(4, 4, 100) == ERR_ARG
+    assert lib.sgg_gemm_fp8_splits(-1, 4, 128, 0) == ERR_ARG and lib.sgg_gemm_fp8_splits(4, 4, 100, 0) == ERR_ARG and lib.sgg_gemm_fp8_splits(4, 4, 128, 9) == ERR_DTYPE
     for M, N, Kp in ((1, 4096, 25088), (256, 4096, 25088), (8192, 8192, 128), (1, 1, 128), (0, 0, 0), (333, 1100, 2048)):
-        s = lib.sgg_gemm_fp8_splits(M, N, Kp)
-        assert 1 <= s <= max(1, Kp // 128), (M, N, Kp, s)
+        for code in (0, 1, 2):
+            s = lib.sgg_gemm_fp8_splits(M, N, Kp, code)
+            assert 1 <= s <= max(1, Kp // 128), (M, N, Kp, s)
     assert lib.sgg_fp8_scale_bytes(1, 1) == 128 and lib.sgg_fp8_scale_bytes(129, 257) == 3 * 256 and lib.sgg_fp8_scale_bytes(0, 5) == 0
 
 
