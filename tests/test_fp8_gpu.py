@@ -183,6 +183,25 @@ def test_product_into_a_strided_buffer_leaves_the_rest(M, K, N, ld):
         assert bool((buf[0] == 9).all()) and bool((buf[M + 1] == 9).all()) and bool((buf[:, :3] == 9).all()) and bool((buf[:, 3 + N:] == 9).all())
 
 
+@pytest.mark.parametrize('M,N', [(4, 64), (20, 64), (100, 64), (4096, 2048), (4096, 4096)])
+def test_operands_near_the_smallest(M, N):
+    """one product per output: exact down to operands of 2^-133 (bf16's smallest), below that exact or zero"""
+    from sgg_amd import ops
+    e = -(112 + torch.arange(N, device=DEV) % 24)                        # down to 2^-135 = e4m3's smallest times the smallest scale
+    x, w = torch.zeros(M, 128, device=DEV), torch.zeros(N, 128, device=DEV)
+    x[:, 0] = 2.0 ** 118
+    w[:, 0] = ((e.clamp(min=-126).int() + 127) << 23).view(torch.float32)
+    w[:, 0] *= ((e - e.clamp(min=-126) + 127).int() << 23).view(torch.float32)
+    A, W = ops.quantize_fp8(x), ops.quantize_fp8(w)
+    want = (A.dequantize()[:1, :1] * W.dequantize()[:, :1].t())
+    assert torch.equal(want[0], ((e.long() + 118 + 1023) << 52).view(torch.float64))
+    for out in (F32, F16, BF16):
+        y = ops.gemm_fp8(A, W, out_dtype=out)
+        exact, low = want.to(out).expand(M, N), e < -133
+        assert torch.equal(y[:, ~low], exact[:, ~low])
+        assert bool(((y[:, low] == exact[:, low]) | (y[:, low] == 0)).all())
+
+
 def test_scales_far_apart_and_zero_operands():
     """blocks of one row 2^60 apart, rows of zeros, a whole zero operand"""
     from sgg_amd import ops
