@@ -1427,6 +1427,7 @@ def clip_grads_(grads, max_norm, grad_scale=1.0, out=None):
         if o is not g and (o.shape != g.shape or not (o.stride() == g.stride() or (o.is_contiguous() and g.is_contiguous()))):
             raise ValueError('sgg_amd: clip_grads_: out %s %s for a gradient %s %s' % (tuple(o.shape), tuple(o.stride()), tuple(g.shape), tuple(g.stride())))
     norm = _clip_call(grads, outs, float(max_norm), float(grad_scale))
-    if outs:
-        torch.autograd.graph.increment_version(outs)          # written through raw pointers
+    told = [o for o in outs if not o.is_inference()]
+    if told:
+        torch.autograd.graph.increment_version(told)          # written through raw pointers
     return norm

@@ -150,6 +150,34 @@ def test_same_bits_every_time_and_in_a_replayed_graph():
         assert torch.equal(norm, n2) and all(torch.equal(a, b) for a, b in zip(out, out2))
 
 
+def test_one_tensor_past_4_gigabytes_on_another_stream():
+    from sgg_amd import ops
+    n = (1 << 32) + 12345
+    g = torch.zeros(n, dtype=F16, device=DEV)
+    at = torch.tensor([0, 5, 1 << 31, (1 << 32) - 1, 1 << 32, n - 1], device=DEV)
+    g[at] = torch.tensor([3.0, -1.0, 2.0, 5.0, -4.0, 7.0], device=DEV).half()
+    want = want_of([g[at]], 2.0, 0.5)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        out = torch.ones(n, dtype=BF16, device=DEV)
+        norm = ops.clip_grads_(g, 2.0, 0.5, out=out)
+    torch.cuda.current_stream().wait_stream(s)
+    check(norm, [out[at]], want)
+    out[at] = 0
+    assert not out.any()
+    del g, out
+    torch.cuda.empty_cache()
+
+
+def test_inference_tensors_are_clipped():
+    from sgg_amd import ops
+    with torch.inference_mode():
+        g = torch.full((100,), 3.0, device=DEV)
+        ops.clip_grads_([g], 1.0)
+        assert abs(float(g.norm()) - 1.0) < 1e-5
+
+
 def test_refusals():
     from sgg_amd import ops
     g = torch.randn(100, device=DEV)

@@ -154,7 +154,7 @@ def check(got, want, tol):
 SIZES = [(1, 1, 1), (1, 128, 128), (2, 100, 5), (1, 4096, 1000), (3, 25088, 300), (16, 1000, 4096), (17, 640, 33), (31, 3000, 100), (32, 2048, 512),
          (33, 1100, 129), (64, 5000, 64), (100, 4096, 700), (128, 128, 128), (127, 257, 129), (256, 12544, 256), (256, 640, 512), (300, 1024, 300),
          (513, 512, 257), (1000, 384, 1000), (1985, 1100, 333), (2048, 896, 2048), (2304, 640, 2300), (4097, 256, 260), (5000, 130, 3), (7, 130, 5000),
-         (24, 25088, 300), (40, 25088, 300), (300, 12544, 200),                        # K slices of each kind
+         (24, 25088, 300), (40, 25088, 300), (300, 12544, 200), (90, 12800, 1900), (700, 12800, 1900), (2500, 25088, 2500),      # K slices of each kind
          (2304, 100, 2300), (2500, 1000, 2450), (2561, 129, 2000),                     # 256 x 128 tiles: one block, several, ragged edges
          (3000, 100, 3000), (3001, 256, 2901), (3000, 385, 3000), (4352, 700, 4500), (2816, 2048, 3328)]   # 256 x 256 tiles
 
@@ -200,6 +200,29 @@ def test_operands_near_the_smallest(M, N):
         exact, low = want.to(out).expand(M, N), e < -133
         assert torch.equal(y[:, ~low], exact[:, ~low])
         assert bool(((y[:, low] == exact[:, low]) | (y[:, low] == 0)).all())
+
+
+@pytest.mark.parametrize('M', [3, 20, 100, 250, 600])
+def test_operands_past_4_gigabytes(M):
+    """W's codes are 4.4 GB (and its f16 source 8.8): a few rows that hold something, the last ones among them"""
+    from sgg_amd import ops
+    N, K = 40001, 110100
+    g = torch.Generator(device=DEV).manual_seed(M)
+    at = torch.tensor([0, 1, 127, 20000, N - 129, N - 2, N - 1], device=DEV)
+    some = (torch.randn(7, K, generator=g, device=DEV) / 300).half()
+    w = torch.zeros(N, K, dtype=F16, device=DEV)
+    w[at] = some
+    W = ops.quantize_fp8(w)
+    del w
+    A = ops.quantize_fp8(torch.randn(M, K, generator=g, device=DEV))
+    few = ops.quantize_fp8(some)
+    for out in (F32, F16):
+        y = ops.gemm_fp8(A, W, out_dtype=out)
+        check(y[:, at], *product(A, few, dtype=out))
+        y[:, at] = 0
+        assert not y.any()
+    del W
+    torch.cuda.empty_cache()
 
 
 def test_scales_far_apart_and_zero_operands():

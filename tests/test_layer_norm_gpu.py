@@ -239,6 +239,29 @@ def test_replayed_graph_equals_eager():
         assert all(torch.equal(a, e) for a, e in zip(out, step()))
 
 
+def test_rows_past_4_gigabytes():
+    """17 GB of bf16 rows; the last ones and some on the way hold something, the others zeros"""
+    from sgg_amd import ops
+    M, C = 540001, 16001
+    at = torch.tensor([0, 134218, 268436, M - 2, M - 1], device='cuda:0')
+    xs, w, b, gs = make(5, C, torch.bfloat16, 5)
+    x = torch.zeros(M, C, dtype=torch.bfloat16, device='cuda:0')
+    x[at] = xs
+    dy = torch.zeros_like(x)
+    dy[at] = gs
+    y, mean, rstd = ops.layer_norm(x, w, b)
+    dx, dw, db = ops.layer_norm_bwd(dy, x, mean, rstd, w)
+    want, tol = reference(xs, w, b, gs, 1e-5)
+    for got, v, t, name in ((y[at], want[0], tol[0], 'y'), (dx[at], want[1], tol[1], 'dx'), (dw, want[2], tol[2], 'dw'), (db, want[3], tol[3], 'db')):
+        check(got, v, t, name)
+    y[at] = b.to(y.dtype)
+    assert bool((y == b.to(y.dtype)).all())
+    dx[at] = 0
+    assert not dx.any()
+    del x, dy, y, dx
+    torch.cuda.empty_cache()
+
+
 def test_refusals():
     from sgg_amd import dense, ops
     x = torch.randn(4, 8, device=DEV)
