@@ -54,11 +54,23 @@ __device__ __forceinline__ float row16_max(float v) {
     return v;
 }
 
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+// 8 elements at any alignment (this chip's 16-byte loads need none)
+template <typename T> __device__ __forceinline__ void load8_any(const T* p, float (&v)[8]) {
+    const u32x4 q = *reinterpret_cast<const u32x4_any*>(p);
+    unpack8<T>(q, v);
+}
+template <> __device__ __forceinline__ void load8_any<float>(const float* p, float (&v)[8]) {
+    const f32x4 a = *reinterpret_cast<const f32x4_any*>(p), b = *reinterpret_cast<const f32x4_any*>(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+
 // One workgroup = a tile of 128 x 128 values; thread (tr, tc) holds rows 8 tr .. 8 tr + 7, columns 8 tc .. 8 tc + 7.  The row form needs the largest
 // magnitude of each row of the tile (16 lanes meet), the transposed form that of each column (LDS), the column sums (a bias gradient) one number per
 // column: all out of one reading, which is what bounds it (8-byte and 16-byte stores, every line of both outputs written whole).
-// Measured: 7936 x 25088 f16 to the row form 115 .. 125 us (600 MB, 4.8 .. 5.2 TB/s: a copy's rate); 7936 x 4096 bf16 to both forms 33 us (130 MB, 3.9 TB/s; the
-// memory's latency at 2000 tiles, five of them per CU), with the column sums 31; one row of 25088 5 us.
+// Measured: 7936 x 25088 f16 to the row form 115 .. 125 us (600 MB, 4.8 .. 5.2 TB/s: a copy's rate); 7936 x 4096 bf16 to both forms 27 us warm, 33 cold
+// (130 MB, 4.8 and 3.9 TB/s); 1985 x 333 f32, rows of no alignment, to both 7 us (element by element 12); one row of 25088 3 us.
 // max() drops NaN, so only infinities need a second look: a tile's rows (columns) are gone over again without them where the maximum is infinite.
 template <typename T, bool ROWS, bool COLS, bool SUM>
 __global__ __launch_bounds__(256) void fp8_quantize_kernel(const T* __restrict__ x, long ldx, long M, int K, unsigned char* __restrict__ rows,
@@ -74,21 +86,23 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(const T* __restrict__
     const int k0 = tk * QB;
     const long RM = slab_rows(M);
     float v[8][8];
-    const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ldx * (long)sizeof(T)) % 16 == 0 && k0 + tc * 8 + 8 <= K;
+    const int left = min(8, K - k0 - tc * 8);
     const T* p0 = x + (m0 + tr * 8) * ldx + k0 + tc * 8;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const bool in = m0 + tr * 8 + i < M;
-        if (in && vec) {
-            load8(p0 + i * ldx, v[i]);
+        if (m0 + tr * 8 + i < M && left == 8) {
+            load8_any(p0 + i * ldx, v[i]);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = in && k0 + tc * 8 + j < K ? Elem<T>::ld(p0 + i * ldx + j) : 0.f;
+            for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+            if (m0 + tr * 8 + i < M)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (j < left) v[i][j] = Elem<T>::ld(p0 + i * ldx + j);
         }
     }
     if constexpr (ROWS) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        auto row_form = [&](int i) {
             float top = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[i][j]));
@@ -101,9 +115,18 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(const T* __restrict__
                 top = row16_max(top);
             }
             const int byte = scale_byte(top);
-            const long m = m0 + tr * 8 + i;
-            if (m < RM) *reinterpret_cast<u32x2*>(rows + ((2L * tk + (tc >> 3)) * RM + m) * 64 + (tc & 7) * 8) = pack_fp8x8(v[i], scale_inv(byte), inf);
-            if (tc == 0) rbyte[tr * 8 + i] = (unsigned char)byte;                        // (rows past M of the last group: blocks of zeros)
+            if (m0 + tr * 8 + i < RM)
+                *reinterpret_cast<u32x2*>(rows + ((2L * tk + (tc >> 3)) * RM + m0 + tr * 8 + i) * 64 + (tc & 7) * 8) = pack_fp8x8(v[i], scale_inv(byte), inf);
+            if (tc == 0) rbyte[tr * 8 + i] = (unsigned char)byte;
+        };
+        if (COLS || m0 + 128 <= M) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) row_form(i);
+        } else {                                                  // few rows: nothing done for those past the end, whose blocks are zeros (one row: 4.6 us against 5.2; no gain with COLS)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (m0 + tr * 8 + i < RM) row_form(i);
+                else if (tc == 0) rbyte[tr * 8 + i] = (unsigned char)scale_byte(0.f);
         }
     }
     if constexpr (COLS) {
@@ -223,8 +246,6 @@ __device__ __forceinline__ void mma_wide(f32x16& acc, const Wide& w, const Wide&
 }
 
 // ---- where results go: fp32 partial outputs of a K slice ([slice][M][N]), or act(sum + bias) in the output's type
-typedef f32x4 f32x4_any __attribute__((aligned(4)));
-typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
 __device__ __forceinline__ void out_st(char* C, long at, int dt, float v) {
     if (dt == SGG_F32) reinterpret_cast<float*>(C)[at] = v;
