@@ -350,7 +350,7 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(const Fp8Args g, const fl
 __device__ __forceinline__ void tile_and_slice(int tilesM, int tilesN, int& tm, int& tn, int& slice) {
     const int tiles = tilesM * tilesN, logical = xcd_remap(blockIdx.x, gridDim.x);
     slice = logical / tiles;
-    // inside a slice, columns of 4 tiles of M at a time (4 against 8 at 7936 x 4096 x 25088: 699 and 714 us; 16: 729)
+    // inside a slice, columns of 4 tiles of M at a time (4, 6 and 8 within 1 %)
     constexpr int GM = 4;
     const int t = logical - slice * tiles, first = t / (GM * tilesN) * GM, h = min(GM, tilesM - first), in = t - first * tilesN;
     tm = first + in % h;
