@@ -10,6 +10,8 @@
 // Scales are bytes (e + 127), 128 rows to a group: byte ((b * G + m / 128) * 32 + m % 32) * 4 + (m / 32) % 4 with G = ceil(M / 128) -- one dword
 // holds the rows r, r + 32, r + 64, r + 96 of a group, i.e. what a lane of the 32-row MFMA fragments needs, picked by the instruction's
 // byte selector.
+#include <atomic>
+
 #include "gemm_args.h"
 
 namespace {
@@ -851,10 +853,12 @@ Fp8Plan fp8_plan(int64_t M, int64_t N, int64_t Kp, bool wide) {
 
 template <auto kernel>
 int fp8_launch(const Fp8Plan& p, int threads, int smem, const Fp8Args& g, float* ws, hipStream_t s) {
-    static bool attr_done = false;
-    if (smem > 65536 && !attr_done) {
+    static std::atomic<unsigned long> told{0};               // devices that know of this kernel's LDS, a bit each
+    int dev = 0;
+    if (smem > 65536 && hipGetDevice(&dev) != hipSuccess) return SGG_ERR_LAUNCH;
+    if (smem > 65536 && !(told.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
         if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, smem) != hipSuccess) return SGG_ERR_LAUNCH;
-        attr_done = true;
+        told.fetch_or(1ul << (dev & 63), std::memory_order_relaxed);
     }
     hipLaunchKernelGGL(kernel, dim3(p.tiles * p.slices), dim3(threads), smem, s, g, ws, p.per, p.slices);
     SGG_CHECK_LAUNCH();
