@@ -14,6 +14,8 @@ normalisation), so the reference's checkpoints load by name.
 
 The kernels run on the GPU only: a CPU tensor raises (there is no fallback path).
 """
+import functools
+
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
@@ -127,6 +129,17 @@ def _row_form(x):
     return x if (K <= 1 or x.stride(1) == 1) and (M <= 1 or x.stride(0) >= K) else x.contiguous()
 
 
+def _gemm_rows(x, w, b, out_dtype):
+    b = None if b is None else b.detach().float().contiguous()
+    return ops._gemm_fp8(x, w, ops._vector(b, w.shape[0], 'dense bias'), out_dtype=out_dtype)
+
+
+def _once_differentiable(backward):
+    """autograd's once_differentiable, which switches the gradient mode and back, only where that is on (create_graph): ~4 us of a small backward"""
+    careful = torch.autograd.function.once_differentiable(backward)
+    return functools.wraps(backward)(lambda ctx, dy: careful(ctx, dy) if torch.is_grad_enabled() else backward(ctx, dy))
+
+
 class _AffineFp8(torch.autograd.Function):
     """y = Q(x) . Q(w)^T + b, dx = Q(dy) . Q(w^T)^T, dw = Q(dy^T) . Q(x^T)^T, db = column sums of dy, Q the 8-bit operand form (ops.quantize_fp8:
     blocks of 128 along each product's own reduction, so x, w and dy are read once and written in both orders).  What the backward
@@ -144,10 +157,10 @@ class _AffineFp8(torch.autograd.Function):
         ctx.save_for_backward(*[t for q in (xt, wt) if q is not None for t in (q.data, q.scale)])
         ctx.kept = tuple(None if q is None else q.shape for q in (xt, wt))
         ctx.types = (x.dtype, w.dtype, b.dtype if b is not None else None)
-        return ops.gemm_fp8(xq, wq, b.detach().float().contiguous() if b is not None else None, out_dtype=out_dtype)
+        return _gemm_rows(xq, wq, b, out_dtype)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once_differentiable
     def backward(ctx, dy):
         saved = iter(ctx.saved_tensors)
         xt, wt = [None if shape is None else ops.Fp8Rows(next(saved), next(saved), shape) for shape in ctx.kept]
@@ -165,9 +178,9 @@ class _AffineFp8(torch.autograd.Function):
             if need_db:
                 db = ops.colsum(dy.contiguous()) if dy.shape[0] else dy.new_zeros(dy.shape[1], dtype=torch.float32)
         if need_dx:
-            dx = ops.gemm_fp8(dq, wt, out_dtype=ctx.types[0])
+            dx = ops._gemm_fp8(dq, wt, out_dtype=ctx.types[0])
         if need_dw:
-            dw = ops.gemm_fp8(dt, xt).to(ctx.types[1])
+            dw = ops._gemm_fp8(dt, xt).to(ctx.types[1])
         if db is not None:
             db = db.to(ctx.types[2])
         return dx, dw, db, None
@@ -187,7 +200,7 @@ def _affine_fp8_rows(x, w, b, out_dtype):
         return _AffineFp8.apply(x, w, b, out_dtype)
     if x.shape[1] != w.shape[1]:
         raise ValueError('dense: inputs %s against weights %s' % (tuple(x.shape), tuple(w.shape)))
-    return ops.gemm_fp8(ops.quantize_fp8(_row_form(x)), ops.quantize_fp8(_row_form(w)), b.detach().float().contiguous() if b is not None else None, out_dtype=out_dtype)
+    return _gemm_rows(ops.quantize_fp8(_row_form(x)), ops.quantize_fp8(_row_form(w)), b, out_dtype)
 
 
 def _affine_rows(x, w, b):
@@ -333,12 +346,11 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once_differentiable
     def backward(ctx, dy):
         x, stats, w = ctx.saved_tensors
         need = ctx.needs_input_grad
-        ops._here(x, 'layer_norm backward')
-        dy = _row_form(dy)                           # (autograd has seen to its shape and type; x and w were checked on the way in)
+        dy = dy if dy.is_contiguous() else _row_form(dy)             # (autograd has seen to shape, type and device; x and w were checked on the way in)
         C, mean = x.shape[1], stats.data_ptr()
         return ops._layer_norm_bwd(dy, max(dy.stride(0), C), x, max(x.stride(0), C), mean, mean + 4 * x.shape[0], None if w is None else w.data_ptr(),
                                    need[0], need[1], need[2]) + (None,)

@@ -1237,7 +1237,8 @@ def _layer_norm_bwd(dy, ld_dy, x, ld, mean, rstd, w, want_dx, want_dw, want_db):
     ws = None
     if want_dw or want_db:
         parts = _lib.load().sgg_layer_norm_bwd_parts(M, C, code)
-        _lib.check(min(parts, 0), 'sgg_layer_norm_bwd_parts')
+        if parts < 0:
+            _lib.check(parts, 'sgg_layer_norm_bwd_parts')
         ws = _ws(2 * C * parts, x.device)
     if want_dx or ws is not None:
         _lib.call('sgg_layer_norm_bwd', dy.data_ptr(), ld_dy, x.data_ptr(), ld, w, mean, rstd, dx.data_ptr() if want_dx else None,
@@ -1332,19 +1333,29 @@ def gemm_fp8(A, W, bias=None, act=ACT_NONE, out_dtype=torch.float32, out=None):
         slabs, R, scales = _fp8_dims(rows, cols)
         if d.dtype != torch.float8_e4m3fn or sc.dtype != torch.uint8 or d.shape != (slabs, R, 64) or sc.numel() != scales:
             raise ValueError('sgg_amd: gemm_fp8: operand [%d, %d] holds %s %s and %d scales' % (rows, cols, d.dtype, tuple(d.shape), sc.numel()))
+        _p(d), _p(sc)
     b = _vector(bias, N, 'gemm_fp8 bias')
-    if out is None:
-        out = torch.empty((M, N), dtype=out_dtype, device=A.data.device)
-    else:
+    if out is not None:
         _here(out, 'gemm_fp8 out')
         if tuple(out.shape) != (M, N):
             raise ValueError('sgg_amd: gemm_fp8: out %s for a [%d, %d] product' % (tuple(out.shape), M, N))
-    ldc, code = _row_matrix(out, 'gemm_fp8 out'), dt(out)
-    Kp = slabs * 64
+    return _gemm_fp8(A, W, b, act, out_dtype, out)
+
+
+def _gemm_fp8(A, W, b=None, act=ACT_NONE, out_dtype=torch.float32, out=None):
+    """gemm_fp8 of operands that quantize_fp8 made; b: address"""
+    (M, K), N, a, w = A.shape, W.shape[0], A.data, W.data
+    if out is None:
+        out, ldc = torch.empty((M, N), dtype=out_dtype, device=a.device), N
+    else:
+        ldc = _row_matrix(out, 'gemm_fp8 out')
+    code, Kp = dt(out), a.shape[0] * 64
     splits = _lib.load().sgg_gemm_fp8_splits(M, N, Kp, code)
-    _lib.check(min(splits, 0), 'sgg_gemm_fp8_splits')
-    ws = _ws(splits * M * N, out.device) if splits > 1 else None
-    _lib.call('sgg_gemm_fp8', _p(A.data), _p(A.scale), _p(W.data), _p(W.scale), b, out.data_ptr(), ldc, M, N, Kp, act, code, _p(ws), _stream())
+    if splits < 0:
+        _lib.check(splits, 'sgg_gemm_fp8_splits')
+    ws = _ws(splits * M * N, a.device) if splits > 1 else None
+    _lib.call('sgg_gemm_fp8', a.data_ptr(), A.scale.data_ptr(), w.data_ptr(), W.scale.data_ptr(), b, out.data_ptr(), ldc, M, N, Kp, act, code,
+              None if ws is None else ws.data_ptr(), _stream())
     return out
 
 
