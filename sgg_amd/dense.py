@@ -154,7 +154,7 @@ class _AffineFp8(torch.autograd.Function):
         need_dx, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         xq, xt = ops.quantize_fp8(xr, 'both') if need_dw else (ops.quantize_fp8(xr), None)
         wq, wt = ops.quantize_fp8(wr, 'both') if need_dx else (ops.quantize_fp8(wr), None)
-        ctx.save_for_backward(*[t for q in (xt, wt) if q is not None for t in (q.data, q.scale)])
+        ctx.save_for_backward(*[q._mem for q in (xt, wt) if q is not None])
         ctx.kept = tuple(None if q is None else q.shape for q in (xt, wt))
         ctx.types = (x.dtype, w.dtype, b.dtype if b is not None else None)
         return _gemm_rows(xq, wq, b, out_dtype)
@@ -163,7 +163,7 @@ class _AffineFp8(torch.autograd.Function):
     @_once_differentiable
     def backward(ctx, dy):
         saved = iter(ctx.saved_tensors)
-        xt, wt = [None if shape is None else ops.Fp8Rows(next(saved), next(saved), shape) for shape in ctx.kept]
+        xt, wt = [None if shape is None else ops.Fp8Rows._of(next(saved), shape) for shape in ctx.kept]
         need_dx, need_dw, need_db = ctx.needs_input_grad[:3]
         need_dx, need_dw = need_dx and wt is not None, need_dw and xt is not None
         dy = _row_form(dy)

@@ -1262,11 +1262,38 @@ def layer_norm_bwd(dy, x, mean, rstd, weight=None, want_dx=True, want_dw=True, w
 
 class Fp8Rows(object):
     """A matrix [M, K] in the 8-bit operand form of include/sgg_hip.h: `data` float8_e4m3fn [slabs of 64 columns, M rounded up to even, 64],
-    `scale` the exponent bytes of its blocks of 128 columns (the kernels' order), `shape` = (M, K)."""
-    __slots__ = ('data', 'scale', 'shape')
+    `scale` the exponent bytes of its blocks of 128 columns (u8, the kernels' order), `shape` = (M, K)."""
+    __slots__ = ('_mem', 'shape')                    # _mem: (data, scale) as given, or one u8 tensor, the scales behind the codes
 
     def __init__(self, data, scale, shape):
-        self.data, self.scale, self.shape = data, scale, tuple(shape)
+        self._mem, self.shape = (data, scale), tuple(shape)
+
+    @classmethod
+    def _of(cls, mem, shape):
+        q = cls.__new__(cls)
+        q._mem, q.shape = mem, shape
+        return q
+
+    @property
+    def data(self):
+        if isinstance(self._mem, tuple):
+            return self._mem[0]
+        slabs, R, _ = _fp8_dims(*self.shape)
+        return self._mem[:slabs * R * 64].view(torch.float8_e4m3fn).view(slabs, R, 64)
+
+    @property
+    def scale(self):
+        if isinstance(self._mem, tuple):
+            return self._mem[1]
+        slabs, R, _ = _fp8_dims(*self.shape)
+        return self._mem[slabs * R * 64:]
+
+    def _at(self):
+        """addresses of codes and scales"""
+        if isinstance(self._mem, tuple):
+            return self._mem[0].data_ptr(), self._mem[1].data_ptr()
+        p, (slabs, R, _) = self._mem.data_ptr(), _fp8_dims(*self.shape)
+        return p, p + slabs * R * 64
 
     def codes(self):
         """-> float8_e4m3fn [M, K rounded up to 128], the rows as rows"""
@@ -1274,7 +1301,7 @@ class Fp8Rows(object):
 
     def exponents(self):
         """-> int32 [M, blocks]: block b of row m stands for its e4m3 values times 2^exponents[m, b]"""
-        M, blocks = self.shape[0], self.data.shape[0] // 2
+        M, blocks = self.shape[0], (self.shape[1] + FP8_BLOCK - 1) // FP8_BLOCK
         e = self.scale.view(blocks, -1, 32, 4).permute(1, 3, 2, 0).reshape(-1, blocks)        # (block, group, r % 32, r / 32) -> rows
         return e[:M].int() - 127
 
@@ -1293,7 +1320,7 @@ def _fp8_dims(M, K):
 
 def _fp8_empty(M, K, device):
     slabs, R, scales = _fp8_dims(M, K)
-    return Fp8Rows(torch.empty((slabs, R, 64), dtype=torch.float8_e4m3fn, device=device), torch.empty(scales, dtype=torch.uint8, device=device), (M, K))
+    return Fp8Rows._of(torch.empty(slabs * R * 64 + scales, dtype=torch.uint8, device=device), (M, K))
 
 
 def quantize_fp8(x, form='rows', colsum=False):
@@ -1311,9 +1338,9 @@ def quantize_fp8(x, form='rows', colsum=False):
     c = _fp8_empty(K, M, x.device) if form != 'rows' else None
     sums = torch.empty(K, dtype=torch.float32, device=x.device) if colsum else None
     ws = _ws((M + 127) // 128 * K, x.device) if colsum else None
-    _lib.call('sgg_fp8_quantize', x.data_ptr(), ld, M, K, r.data.data_ptr() if r else None, r.scale.data_ptr() if r else None,
-              c.data.data_ptr() if c else None, c.scale.data_ptr() if c else None, sums.data_ptr() if colsum else None, ws.data_ptr() if colsum else None,
-              code, _stream())
+    (rd, rs), (cd, cs) = r._at() if r else (None, None), c._at() if c else (None, None)
+    _lib.call('sgg_fp8_quantize', x.data_ptr(), ld, M, K, rd, rs, cd, cs, sums.data_ptr() if colsum else None, ws.data_ptr() if colsum else None, code,
+              _stream())
     out = r if c is None else c if r is None else (r, c)
     return (out, sums) if colsum else out
 
@@ -1327,10 +1354,16 @@ def gemm_fp8(A, W, bias=None, act=ACT_NONE, out_dtype=torch.float32, out=None):
     if W.shape[1] != K:
         raise ValueError('sgg_amd: gemm_fp8: %s . %s^T' % (A.shape, W.shape))
     for q in (A, W):
-        d, sc, (rows, cols) = q.data, q.scale, q.shape
+        rows, cols = q.shape
+        slabs, R, scales = _fp8_dims(rows, cols)
+        if not isinstance(q._mem, tuple):
+            _here(q._mem, 'gemm_fp8')
+            if q._mem.numel() != slabs * R * 64 + scales:
+                raise ValueError('sgg_amd: gemm_fp8: operand [%d, %d] of %d bytes' % (rows, cols, q._mem.numel()))
+            continue
+        d, sc = q._mem
         _here(d, 'gemm_fp8')
         _here(sc, 'gemm_fp8')
-        slabs, R, scales = _fp8_dims(rows, cols)
         if d.dtype != torch.float8_e4m3fn or sc.dtype != torch.uint8 or d.shape != (slabs, R, 64) or sc.numel() != scales:
             raise ValueError('sgg_amd: gemm_fp8: operand [%d, %d] holds %s %s and %d scales' % (rows, cols, d.dtype, tuple(d.shape), sc.numel()))
         _p(d), _p(sc)
@@ -1343,19 +1376,18 @@ def gemm_fp8(A, W, bias=None, act=ACT_NONE, out_dtype=torch.float32, out=None):
 
 
 def _gemm_fp8(A, W, b=None, act=ACT_NONE, out_dtype=torch.float32, out=None):
-    """gemm_fp8 of operands that quantize_fp8 made; b: address"""
-    (M, K), N, a, w = A.shape, W.shape[0], A.data, W.data
+    """gemm_fp8 of operands that were checked or that quantize_fp8 made; b: address"""
+    (M, K), N = A.shape, W.shape[0]
     if out is None:
-        out, ldc = torch.empty((M, N), dtype=out_dtype, device=a.device), N
+        out, ldc = torch.empty((M, N), dtype=out_dtype, device=(A._mem[0] if isinstance(A._mem, tuple) else A._mem).device), N
     else:
         ldc = _row_matrix(out, 'gemm_fp8 out')
-    code, Kp = dt(out), a.shape[0] * 64
+    code, Kp, (a, sa), (w, sw) = dt(out), (K + 127) // 128 * 128, A._at(), W._at()
     splits = _lib.load().sgg_gemm_fp8_splits(M, N, Kp, code)
     if splits < 0:
         _lib.check(splits, 'sgg_gemm_fp8_splits')
-    ws = _ws(splits * M * N, a.device) if splits > 1 else None
-    _lib.call('sgg_gemm_fp8', a.data_ptr(), A.scale.data_ptr(), w.data_ptr(), W.scale.data_ptr(), b, out.data_ptr(), ldc, M, N, Kp, act, code,
-              None if ws is None else ws.data_ptr(), _stream())
+    ws = _ws(splits * M * N, out.device) if splits > 1 else None
+    _lib.call('sgg_gemm_fp8', a, sa, w, sw, b, out.data_ptr(), ldc, M, N, Kp, act, code, None if ws is None else ws.data_ptr(), _stream())
     return out
 
 

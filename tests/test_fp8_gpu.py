@@ -431,6 +431,12 @@ def test_refusals():
                 ops.Fp8Rows(A.data.view(torch.uint8), A.scale, (4, 256))):
         with pytest.raises(ValueError):                                   # an operand whose memory is not its shape's
             ops.gemm_fp8(bad, bad)
+    by_hand = ops.Fp8Rows(A.data, A.scale, A.shape)
+    assert torch.equal(ops.gemm_fp8(by_hand, A), ops.gemm_fp8(A, by_hand))
+    A.shape = (1000, 256)
+    with pytest.raises(ValueError):
+        ops.gemm_fp8(A, A)
+    A.shape = (4, 256)
     with pytest.raises(ValueError):
         ops.gemm_fp8(A, A, torch.zeros(5, device=DEV))
     with pytest.raises(TypeError):
