@@ -1428,21 +1428,13 @@ def _clip_call(grads, outs, max_norm, grad_scale):
         ocode = [_DT.get(o.dtype, -1) for o in outs]
     if -1 in code or -1 in ocode:
         raise TypeError('sgg_amd: clipping: float32 / bfloat16 / float16 tensors only')
-    if outs is not None:
-        # every tensor is written by workgroups of its own: no two of them may share memory (one given twice would be scaled twice)
-        mem = [(p, p + k * (4 if c == SGG_F32 else 2)) for p, k, c in zip(ptr, num, code) if k]
-        if optr is not ptr:                                      # (an output that IS its gradient: in place)
-            mem += [(o, o + k * (4 if d == SGG_F32 else 2)) for p, o, k, c, d in zip(ptr, optr, num, code, ocode) if k and (o != p or c != d)]
-        mem.sort()
-        end = 0
-        for lo, hi in mem:
-            if lo < end:
-                raise ValueError('sgg_amd: clip_grads_: two of the tensors share memory')
-            end = hi
     ptrs, ints = ctypes.c_void_p * n, ctypes.c_int * n
     g, d = ptrs(*ptr), ints(*code)
     o, od = (None, None) if outs is None else (g, d) if optr is ptr else (ptrs(*optr), ints(*ocode))
-    _lib.call('sgg_clip_grads', g, o, (ctypes.c_int64 * n)(*num), d, od, n, max_norm, grad_scale, ws.data_ptr(), norm.data_ptr(), _stream())
+    try:
+        _lib.call('sgg_clip_grads', g, o, (ctypes.c_int64 * n)(*num), d, od, n, max_norm, grad_scale, ws.data_ptr(), norm.data_ptr(), _stream())
+    except ValueError as e:                                      # what else it refuses was seen to above
+        raise ValueError('sgg_amd: clip_grads_: two of the tensors share memory (or they hold 2^44 elements)') from e
     return norm
 
 
@@ -1464,13 +1456,17 @@ def clip_grads_(grads, max_norm, grad_scale=1.0, out=None):
     outs = grads if out is None else _grad_list(out, 'clip_grads_ out')
     if len(outs) != len(grads):
         raise ValueError('sgg_amd: clip_grads_: %d gradients, %d outputs' % (len(grads), len(outs)))
-    for g, o in zip(grads, outs):
-        if not _dense_layout(g):
+    for g in grads:
+        if not (g.is_contiguous() or _dense_layout(g)):
             raise ValueError('sgg_amd: clip_grads_: gradient of shape %s has gaps or overlaps (strides %s)' % (tuple(g.shape), tuple(g.stride())))
-        if o is not g and (o.shape != g.shape or not (o.stride() == g.stride() or (o.is_contiguous() and g.is_contiguous()))):
-            raise ValueError('sgg_amd: clip_grads_: out %s %s for a gradient %s %s' % (tuple(o.shape), tuple(o.stride()), tuple(g.shape), tuple(g.stride())))
+    if outs is not grads:
+        for g, o in zip(grads, outs):
+            if o.shape != g.shape or not ((o.is_contiguous() and g.is_contiguous()) or o.stride() == g.stride()):
+                raise ValueError('sgg_amd: clip_grads_: out %s %s for a gradient %s %s' % (tuple(o.shape), tuple(o.stride()), tuple(g.shape), tuple(g.stride())))
     norm = _clip_call(grads, outs, float(max_norm), float(grad_scale))
-    told = [o for o in outs if not o.is_inference()]
-    if told:
-        torch.autograd.graph.increment_version(told)          # written through raw pointers
+    if outs:                                                  # written through raw pointers
+        try:
+            torch.autograd.graph.increment_version(outs)
+        except RuntimeError:                                  # inference tensors among them, which have no versions
+            torch.autograd.graph.increment_version([o for o in outs if not o.is_inference()])
     return norm

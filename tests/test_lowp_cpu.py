@@ -69,7 +69,9 @@ def test_clip_entry_refuses():
     def c(g=ptr, out=ptr, n=n, gd=f32, od=f32, count=2, max_norm=1.0, ws=P, norm=P):
         return lib.sgg_clip_grads(g, out, n, gd, od, count, max_norm, 1.0, ws, norm, None)
     for bad in (dict(g=None), dict(g=null), dict(out=null), dict(n=None), dict(n=neg), dict(gd=None), dict(od=None), dict(count=-1), dict(max_norm=-1.0),
-                dict(max_norm=float('nan')), dict(ws=None), dict(norm=None), dict(n=(ctypes.c_int64 * 2)(1 << 62, 1 << 62))):
+                dict(max_norm=float('nan')), dict(ws=None), dict(norm=None), dict(n=(ctypes.c_int64 * 2)(1 << 62, 1 << 62)),
+                dict(g=(ctypes.c_void_p * 2)(P, P), out=(ctypes.c_void_p * 2)(P, P)), dict(g=(ctypes.c_void_p * 2)(P, P + 16), out=(ctypes.c_void_p * 2)(P, P + 16)),
+                dict(out=(ctypes.c_void_p * 2)(P + 4, 2 * P)), dict(gd=(ctypes.c_int * 2)(1, 1), od=(ctypes.c_int * 2)(2, 1))):          # shared memory
         assert c(**bad) == ERR_ARG, bad
     assert c(gd=odd) == ERR_DTYPE and c(od=odd) == ERR_DTYPE
     assert lib.sgg_clip_grads_parts(-1) == ERR_ARG and 0 < lib.sgg_clip_grads_parts(0) <= lib.sgg_clip_grads_parts(1000)
