@@ -423,8 +423,13 @@ int sgg_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ldx
  * reading of x.  Either form may be NULL (with its scales).  rows, cols 16-byte aligned, the scales 4-byte.
  * colsum f32[K] (or NULL; only with `cols`): the column sums of x (a bias gradient of x = dY), added in a fixed order; colsum_ws
  * f32[ceil(M / 128) * K] then.
- * gemm_fp8: C[m][n] = act(sum_k A[m][k] W[n][k] + bias[n]), fp32 accumulation, one rounding to out_dtype; bias f32[N] or NULL; ldc in
- * elements; ws f32[splits * M * N] when sgg_gemm_fp8_splits(M, N, Kp, out_dtype) is more than 1 (the K slices are added in a fixed order). */
+ * gemm_fp8: C[m][n] = act(sum_k A[m][k] W[n][k] + bias[n]), rounded once to out_dtype; bias f32[N] or NULL; ldc in elements; ws
+ * f32[splits * M * N] when sgg_gemm_fp8_splits(M, N, Kp, out_dtype) is more than 1 (the K slices are added in a fixed order).  What is summed:
+ *   out_dtype f32, or M <= 32: whole products, fp32 sums.  An operand's value below 2^-133 counts as 0 or itself, from 2^128 on as infinity.
+ *   otherwise (a 16-bit out_dtype, M > 32): the 8-bit matrix pipe.  A product may be cut, toward zero, at 2^-13 of the largest among its 8 columns
+ *   8 i .. 8 i + 7 (for that, operands below 2^-6 of their block's scale count as 2^-6 of it); fp32 sums of what is left.  Where the terms
+ *   of an output cancel the cut does not shrink with it: ask for an f32 output where that matters.
+ * So the sums of one row in a 16-bit output may differ in their last bits between M <= 32 and M > 32. */
 int64_t sgg_fp8_scale_bytes(int64_t rows, int64_t K);
 int sgg_fp8_quantize(const void* x, int64_t ldx, int64_t M, int64_t K, void* rows, void* rows_scale, void* cols, void* cols_scale, float* colsum,
                      float* colsum_ws, int dtype, void* stream);

@@ -30,8 +30,8 @@ from . import ops
 #         unnormalised discriminator whose activations pass 65504 overflows the hi half: measured, tools/dbg_gan.py), and at the GAN's
 #         shapes the split passes cost what the faster products gain (bench.py --mode gqa_gan: 72 ms either way) -- opt-in;
 #   'f16' operands rounded to f16 once, fp32 accumulate (the SGG head's default mode; for the GAN an accuracy trade the caller opts into);
-#   'fp8' operands rounded to 8-bit floating point with a power-of-two scale per 128 values of the reduction, fp32 accumulate, forward and
-#         both gradients (affine_fp8): a relative rounding of 2^-4 per operand value -- for networks trained in it or served from it.
+#   'fp8' operands rounded to 8-bit floating point with a power-of-two scale per 128 values of the reduction, forward and both gradients
+#         (affine_fp8), f32 results from fp32 sums: a relative rounding of 2^-4 per operand value -- for networks trained in it or served from it.
 _COMPUTE = ['f32']
 
 
@@ -187,8 +187,9 @@ class _AffineFp8(torch.autograd.Function):
 
 
 def affine_fp8(x, weight, bias=None, out_dtype=None):
-    """x [..., K] (f32 / bf16 / f16) -> [..., N] = x . weight^T + bias in 8-bit floating point (ops.gemm_fp8), out_dtype (default x's type);
-    differentiable in all three, the gradients' products in 8 bits too.  What set_compute('fp8') makes of affine / conv2d."""
+    """x [..., K] (f32 / bf16 / f16) -> [..., N] = x . weight^T + bias in 8-bit floating point (ops.gemm_fp8, whose sums are whole in fp32 only for f32
+    results and up to 32 rows), out_dtype (default x's type); differentiable in all three, the gradients' products in 8 bits too: dx in x's type,
+    the weight's always through f32.  What set_compute('fp8') makes of affine / conv2d, with f32 results."""
     _need_gpu(x)
     if x.dim() == 2:                                 # (no views in autograd's graph: ~10 us of the host's each way)
         return _affine_fp8_rows(x, weight, bias, out_dtype or x.dtype)
