@@ -205,10 +205,10 @@ def _affine_fp8_rows(x, w, b, out_dtype):
 
 
 def _affine_rows(x, w, b):
-    """the product of a row matrix in the file's arithmetic (columns of x past w's are zero: a padded patch matrix)"""
+    """the product of a row matrix in the file's arithmetic"""
     if _COMPUTE[0] != 'fp8':
         return _Affine.apply(x, w, b)
-    return _affine_fp8_rows(x, w if w.shape[1] == x.shape[1] else F.pad(w, (0, x.shape[1] - w.shape[1])), b, torch.float32)
+    return _affine_fp8_rows(x, w, b, torch.float32)
 
 
 def affine(x, weight, bias=None):

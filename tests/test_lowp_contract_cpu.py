@@ -1,0 +1,34 @@
+"""What the 8-bit layers, layer norm and clipping refuse or leave to others before any kernel is launched: the launches are stubs here, on the CPU."""
+import pytest
+import torch
+
+
+class Form(object):
+    """stands for an operand form"""
+    def __init__(self, t):
+        self._mem, self.shape = t, tuple(t.shape)
+
+
+@pytest.fixture
+def stubbed(monkeypatch):
+    """dense with products that multiply in torch: what reaches them was let through"""
+    from sgg_amd import dense, ops
+    monkeypatch.setattr(dense, '_need_gpu', lambda x: None)
+    monkeypatch.setattr(ops, 'quantize_fp8', lambda x, form='rows', colsum=False: Form(x) if form == 'rows' else (Form(x), Form(x.t())))
+    monkeypatch.setattr(ops, '_vector', lambda t, n, what: None)
+    monkeypatch.setattr(ops, '_gemm_fp8', lambda a, w, b=None, act=0, out_dtype=torch.float32, out=None: a._mem @ w._mem.t())
+    prev = dense.set_compute('fp8')
+    yield dense
+    dense.set_compute(prev)
+
+
+@pytest.mark.parametrize('grad', [True, False])
+def test_fp8_layers_refuse_another_width(stubbed, grad):
+    lin = stubbed.Linear(100, 5)
+    with torch.set_grad_enabled(grad):
+        assert lin(torch.randn(3, 100)).shape == (3, 5)
+        for width in (64, 96, 99, 101, 130):
+            with pytest.raises(ValueError):
+                lin(torch.randn(3, width))
+            with pytest.raises(ValueError):
+                stubbed.affine(torch.randn(2, 3, width), lin.weight)
