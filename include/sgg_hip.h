@@ -406,6 +406,8 @@ int sgg_sgd_multi(float* const* p, const void* const* g, float* const* momentum_
 /* ---- layer normalisation over the last axis (beside the batch / instance normalisations of the GAN's layers) ----
  * y = (x - mean) / sqrt(var + eps) * w + b per row, var = mean((x - mean)^2); x [M, C] with row stride ldx, y [M, C] contiguous, both `dtype`;
  * w, b f32[C] or NULL; mean, rstd f32[M] (what the backward reads), both or neither NULL; 1 <= C <= SGG_LAYER_NORM_MAX, eps > 0.
+ * Rows far from zero keep their differences: the mean's rounding does not enter y (a constant row gives b).  A row with a NaN or an infinity, and a bf16
+ * row whose sum passes 3.4e38, gives NaN.  bwd takes mean as fwd wrote it and centres x by what its rounding to f32 has left, too.
  * bwd: dx [M, C] contiguous (or NULL), dw, db f32[C] (or NULL), overwritten; dw_j = sum dy xhat, db_j = sum dy, added in a fixed order.
  * ws: f32[2 * C * sgg_layer_norm_bwd_parts(M, C, dtype)] when dw or db is wanted. */
 #define SGG_LAYER_NORM_MAX 16384

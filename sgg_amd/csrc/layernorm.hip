@@ -1,17 +1,21 @@
 // Layer normalisation over the last axis, forward and backward (f32 / bf16 / f16 rows, fp32 weight, bias, statistics and sums).
 //   mu = sum_j x_j / C,  v = sum_j (x_j - mu)^2 / C,  r = 1 / sqrt(v + eps),  xh = (x - mu) r,  y = xh w + b
 //   g = dy w,  dx = r (g - mean_j g - xh mean_j(g xh)),  dw_j = sum_i dy_ij xh_ij,  db_j = sum_i dy_ij
-// The variance is summed from the centred values (x - mu), never as E[x^2] - mu^2: rows far from zero lose nothing.
+// Rows far from zero lose nothing: the mean comes from a sum without fp32's rounding (LnSum) and is subtracted as two floats -- an fp32 sum's error, a
+// few 2^-24 of the MEAN, would enter every x - mu and be multiplied by r, up to 316: constant rows of 1e6 came out 1.0 from 0 --, the variance
+// is summed from the centred values, never as E[x^2] - mu^2, and the backward, which gets the mean as one float, centres once more by the mean of what is left.
 //
 // Memory-bound both ways (8 .. 24 operations per element against 4 .. 12 bytes), so every row is read once and stays in registers between its
 // sums and its result, and a workgroup walks many rows: w, b -- 8 bytes per column, twice a 16-bit row's -- and the column sums of dw, db live in
 // registers over all of them, and the next row's loads are in flight while this one is reduced.  A lane owns pieces of 8 consecutive columns.  How many
 // lanes share a row follows from C alone (LnShape): 8 .. 64 lanes of one wave up to 512 columns (several rows per wave: short rows would
 // leave lanes idle), then 1 .. 16 waves with two pieces per lane, which is what the registers of the backward hold.
-// Measured (a copy reaches 4.9 TB/s): 65536 x 4096 bf16 forward 194 us (5.5 TB/s), backward 334 us (4.8); 12345 x 1001 f32 20 and 27 us (4.9, 5.4);
-// 7936 x 512 f16, 8 MB, 7 and 9 us; the join of the column sums 4 .. 7 us; one row of 512 2 us.
+// Measured (a copy reaches 4.9 TB/s), the backward with the join of its column sums, 4 .. 7 us: 65536 x 4096 bf16 forward 197 us (5.5 TB/s), backward 308 us
+// (5.2); 12345 x 1001 f32 19 and 35 us (5.2, 4.3); 7936 x 512 f16, 8 MB, 5.6 and 11.7 us; one row of 512 2 us.
 // Rows of any alignment are loaded 16 bytes at a time (this chip's global loads need no alignment); only a row's last, partial piece goes
 // element by element.
+#include <type_traits>
+
 #include "common.h"
 
 namespace {
@@ -99,25 +103,49 @@ __device__ __forceinline__ void load_columns(const float* p, const L& at, float 
     }
 }
 
-// sum over the lanes of a row; every lane of the row gets it.  red: WAVES floats of LDS, a set of its own per call inside one row (no lane can be two
-// calls ahead of another: the barriers in between)
-template <typename S>
-__device__ __forceinline__ float row_sum(float v, float* red) {
-    if constexpr (S::LPR == 64) {
-        v = wave_sum(v);
-        if constexpr (S::WPR > 1) {
-            const int wave = threadIdx.x >> 6;
-            if ((threadIdx.x & 63) == 0) red[wave] = v;
-            __syncthreads();
-            v = 0.f;
-#pragma unroll
-            for (int i = 0; i < S::WPR; ++i) v += red[wave / S::WPR * S::WPR + i];
-        }
-    } else {
-#pragma unroll
-        for (int o = S::LPR / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+// v of another lane, by DPP (lanes that `rmask` leaves out get 0)
+template <int CTRL, int RMASK = 0xF> __device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, RMASK, 0xF, false));
+}
+template <int CTRL, int RMASK = 0xF> __device__ __forceinline__ double dpp(double v) {
+    return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, RMASK, 0xF, false),
+                            __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, RMASK, 0xF, false));
+}
+__device__ __forceinline__ float lane63(float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63)); }
+__device__ __forceinline__ double lane63(double v) {
+    return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), 63), __builtin_amdgcn_readlane(__double2loint(v), 63));
+}
+// sum over each W neighbouring lanes (a power of two); every one of them gets it
+template <int W, typename F> __device__ __forceinline__ F lanes_sum(F v) {
+    if constexpr (W >= 2) v += dpp<0xB1>(v);                     // quad_perm [1,0,3,2]
+    if constexpr (W >= 4) v += dpp<0x4E>(v);                     // quad_perm [2,3,0,1]
+    if constexpr (W >= 8) v += dpp<0x141>(v);                    // row_half_mirror
+    if constexpr (W >= 16) v += dpp<0x140>(v);                   // row_mirror
+    if constexpr (W == 32) v += __shfl_xor(v, 16, 64);
+    if constexpr (W == 64) {
+        v += dpp<0x142, 0xA>(v);                                 // row_bcast15 into rows 1, 3
+        v += dpp<0x143, 0xC>(v);                                 // row_bcast31 into rows 2, 3: lane 63 holds the sum
+        v = lane63(v);
     }
     return v;
+}
+
+// N sums at once over the lanes of a row; every lane of the row gets them.  red: N x WAVES values of LDS that no call one barrier earlier or later uses (no
+// lane can be two barriers ahead of another)
+template <typename S, int N, typename F>
+__device__ __forceinline__ void row_sums(F (&v)[N], F* red) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = lanes_sum<S::LPR>(v[k]);
+    if constexpr (S::WPR > 1) {                                  // (LPR = 64: one value per wave)
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        if (lane == 0) {
+#pragma unroll
+            for (int k = 0; k < N; ++k) red[k * S::WAVES + wave] = v[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = lanes_sum<S::WPR>(red[k * S::WAVES + wave / S::WPR * S::WPR + lane % S::WPR]);
+    }
 }
 
 template <typename S> struct LnLane {
@@ -134,16 +162,40 @@ template <typename S> struct LnLane {
     }
 };
 
+// The type a row's sum is held in.  Values of 16 bits that lie within a factor 4 add up in fp32 without any rounding: 8 (bf16) or 11 significand bits,
+// 2 for the factor, 14 or 11 for as many columns, 24 in all; and where a row is wider than a factor 4, its spread is max|x| / sqrt(2 C) or more and
+// fp32's rounding, 6e-7 max|x|, nothing beside it.  All others take 64 bits (65536 x 4096 bf16 in 64 bits: 201 us, 197 this way;
+// 100000 x 200 f16 20.3 and 17.7).
+template <typename T, int CAP> struct LnSum { using type = double; };
+template <int CAP> struct LnSum<bf16_t, CAP> { using type = float; };
+template <int CAP> struct LnSum<f16_t, CAP> { using type = std::conditional_t<(CAP <= 2048), float, double>; };
+constexpr float LN_TINY = 0x1p-80f;
+
+// the mean as two floats from the sum: the quotient itself (of a constant row the constant), and what its rounding leaves
+__device__ __forceinline__ void ln_mean(double s, double C, double invC, float& mu, float& rest) {
+    double m = s * invC;
+    m = fma(fma(-m, C, s), invC, m);
+    mu = (float)m;
+    rest = (float)(m - (double)mu);
+}
+__device__ __forceinline__ void ln_mean(float s, float C, float invC, float& mu, float& rest) {
+    mu = s * invC;
+    mu = fmaf(fmaf(-mu, C, s), invC, mu);
+    rest = fmaf(-mu, C, s) * invC;
+}
+
 template <typename T, typename S>
 __global__ __launch_bounds__(S::THREADS) void ln_fwd_kernel(const T* __restrict__ x, long ldx, const float* __restrict__ w, const float* __restrict__ b,
                                                             T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd, long M, int C, float eps) {
-    __shared__ float red[2][S::WAVES];
+    using Sum = typename LnSum<T, S::CAP>::type;
+    __shared__ Sum red_mean[S::WAVES];
+    __shared__ float red_var[2][S::WAVES];
     const LnLane<S> at(C);
     float wv[S::NV][8], bv[S::NV][8];
     load_columns(w, at, 1.f, wv);
     load_columns(b, at, 0.f, bv);
     const long step = (long)gridDim.x * S::GROUPS;
-    const float invC = 1.f / (float)C;
+    const Sum invC = (Sum)1 / (Sum)C;
     Piece<T> p[S::NV];
     // every workgroup's trip count is uniform (barriers inside): a group past the last row works on row M - 1 again and stores nothing
     long row0 = (long)blockIdx.x * S::GROUPS;
@@ -157,14 +209,14 @@ __global__ __launch_bounds__(S::THREADS) void ln_fwd_kernel(const T* __restrict_
     for (; row0 < M; row0 += step) {
         const long row = row0 + at.group;
         float v[S::NV][8];
-        float s = 0.f;
+        Sum sum[1] = {};
 #pragma unroll
         for (int i = 0; i < S::NV; ++i) {
             if (at.n[i] > 0) p[i].get(v[i]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 v[i][j] = j < at.n[i] ? v[i][j] : 0.f;
-                s += v[i][j];
+                sum[0] += (Sum)v[i][j];
             }
         }
         if (row0 + step < M) {                                    // the next row's loads
@@ -173,16 +225,41 @@ __global__ __launch_bounds__(S::THREADS) void ln_fwd_kernel(const T* __restrict_
             for (int i = 0; i < S::NV; ++i)
                 if (at.n[i] > 0) p[i].load(xr + at.col[i], at.n[i]);
         }
-        const float mu = row_sum<S>(s, red[0]) * invC;
-        s = 0.f;
+        row_sums<S>(sum, red_mean);
+        float mu, rest;
+        ln_mean(sum[0], (Sum)C, invC, mu, rest);
+        float sq[1] = {0.f};
 #pragma unroll
         for (int i = 0; i < S::NV; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                v[i][j] = j < at.n[i] ? v[i][j] - mu : 0.f;
-                s = fmaf(v[i][j], v[i][j], s);
+                v[i][j] = j < at.n[i] ? (v[i][j] - mu) - rest : 0.f;
+                sq[0] = fmaf(v[i][j], v[i][j], sq[0]);
             }
-        const float r = 1.0f / sqrtf(row_sum<S>(s, red[1]) * invC + eps);
+        row_sums<S>(sq, red_var[0]);
+        float r = 1.0f / sqrtf(sq[0] * (float)invC + eps);
+        if constexpr (!std::is_same_v<T, f16_t>) {
+            // differences past 2^57 or so, whose squares fp32 does not hold: once more, scaled (eps is nothing beside them).  Every lane of a wave, and of
+            // a workgroup whose waves share rows, has to come along
+            bool again = __any(r == 0.f);
+            if constexpr (S::WPR > 1 && S::GROUPS > 1)
+#pragma unroll
+                for (int g = 0; g < S::WAVES; g += S::WPR) {
+                    float t = 0.f;
+#pragma unroll
+                    for (int i = 0; i < S::WPR; ++i) t += red_var[0][g + i];
+                    again = again || __builtin_isinf(t);
+                }
+            if (again) {
+                float tq[1] = {0.f};
+#pragma unroll
+                for (int i = 0; i < S::NV; ++i)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) tq[0] = fmaf(v[i][j] * LN_TINY, v[i][j] * LN_TINY, tq[0]);
+                row_sums<S>(tq, red_var[1]);
+                if (r == 0.f) r = LN_TINY / sqrtf(tq[0] * (float)invC);
+            }
+        }
         if (row < M) {
 #pragma unroll
             for (int i = 0; i < S::NV; ++i) {
@@ -199,12 +276,13 @@ __global__ __launch_bounds__(S::THREADS) void ln_fwd_kernel(const T* __restrict_
     }
 }
 
-// dx and this workgroup's column sums of dw, db (ws[block][2][C]); DX / DW: which of the two are wanted
+// dx and this workgroup's column sums of dw, db (ws[block][2][C]); DX / DW: which of the two are wanted.  With u = (x - mean) r and a = mean_j u (what the
+// mean's rounding to a float has left): xh = u - a, mean_j(g xh) = mean_j(g u) - a mean_j g, all of a row's sums in one go
 template <typename T, typename S, bool DX, bool DW>
 __global__ __launch_bounds__(S::THREADS) void ln_bwd_kernel(const T* __restrict__ dy, long ld_dy, const T* __restrict__ x, long ldx,
                                                             const float* __restrict__ w, const float* __restrict__ mean, const float* __restrict__ rstd,
                                                             T* __restrict__ dx, float* __restrict__ ws, long M, int C) {
-    __shared__ float red[2][S::WAVES];
+    __shared__ float red[2][3 * S::WAVES];                    // (rows in turn: one barrier per row)
     __shared__ float fold[DW && S::GROUPS > 1 ? S::GROUPS * S::CAP : 1];
     const LnLane<S> at(C);
     float wv[S::NV][8], aw[S::NV][8] = {}, ab[S::NV][8] = {};
@@ -227,43 +305,53 @@ __global__ __launch_bounds__(S::THREADS) void ln_bwd_kernel(const T* __restrict_
     };
     long row0 = (long)blockIdx.x * S::GROUPS;
     if (row0 < M) fetch(row0 + at.group);
-    for (; row0 < M; row0 += step) {
+    int odd = 0;
+    for (; row0 < M; row0 += step, odd ^= 1) {
         const long row = row0 + at.group;
         const float mu = mu_n, r = r_n;
-        float xh[S::NV][8], g[S::NV][8];
-        float s1 = 0.f, s2 = 0.f;
+        float u[S::NV][8], d[S::NV][8];
+        float s[DX ? 3 : 1] = {};
 #pragma unroll
         for (int i = 0; i < S::NV; ++i) {
             if (at.n[i] > 0) {
-                px[i].get(xh[i]);
-                pg[i].get(g[i]);
+                px[i].get(u[i]);
+                pg[i].get(d[i]);
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const bool in = j < at.n[i] && row < M;             // (a row past the end adds nothing)
-                xh[i][j] = in ? (xh[i][j] - mu) * r : 0.f;
-                const float d = in ? g[i][j] : 0.f;
-                if constexpr (DW) {
-                    aw[i][j] = fmaf(d, xh[i][j], aw[i][j]);
-                    ab[i][j] += d;
-                }
+                u[i][j] = in ? (u[i][j] - mu) * r : 0.f;
+                d[i][j] = in ? d[i][j] : 0.f;
+                s[0] += u[i][j];
                 if constexpr (DX) {
-                    g[i][j] = d * wv[i][j];
-                    s1 += g[i][j];
-                    s2 = fmaf(g[i][j], xh[i][j], s2);
+                    const float g = d[i][j] * wv[i][j];
+                    s[1] += g;
+                    s[2] = fmaf(g, u[i][j], s[2]);
                 }
             }
         }
         if (row0 + step < M) fetch(row + step);
+        row_sums<S>(s, red[odd]);
+        const float a = s[0] * invC;
+#pragma unroll
+        for (int i = 0; i < S::NV; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                u[i][j] -= a;
+                asm("" : "+v"(d[i][j]));                          // (d w is multiplied again below: kept over the sums, it would spill at 1024 threads)
+                if constexpr (DW) {
+                    aw[i][j] = fmaf(d[i][j], u[i][j], aw[i][j]);
+                    ab[i][j] += d[i][j];
+                }
+            }
         if constexpr (DX) {
-            s1 = row_sum<S>(s1, red[0]) * invC;
-            s2 = row_sum<S>(s2, red[1]) * invC;
+            const float s1 = s[1] * invC, s2 = s[2] * invC - a * s1;
             if (row < M) {
 #pragma unroll
                 for (int i = 0; i < S::NV; ++i) {
                     float o[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) o[j] = r * (g[i][j] - s1 - xh[i][j] * s2);
+                    for (int j = 0; j < 8; ++j) o[j] = r * (d[i][j] * wv[i][j] - s1 - u[i][j] * s2);
                     if (at.n[i] > 0) Piece<T>::store(dx + row * C + at.col[i], o, at.n[i]);
                 }
             }
