@@ -19,6 +19,7 @@ import functools
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from . import ops
 
@@ -134,6 +135,12 @@ def _gemm_rows(x, w, b, out_dtype):
     return ops._gemm_fp8(x, w, ops._vector(b, w.shape[0], 'dense bias'), out_dtype=out_dtype)
 
 
+def _forward_mode():
+    """inside forward_ad.dual_level(): a layer then always goes through its autograd function, which has no forward derivative and says so where an
+    input carries a tangent (no_grad does not switch forward mode off; the kernels alone would drop the tangent without a word)"""
+    return forward_ad._current_level >= 0
+
+
 def _once_differentiable(backward):
     """autograd's once_differentiable, which switches the gradient mode and back, only where that is on (create_graph): ~4 us of a small backward"""
     careful = torch.autograd.function.once_differentiable(backward)
@@ -197,7 +204,7 @@ def affine_fp8(x, weight, bias=None, out_dtype=None):
 
 
 def _affine_fp8_rows(x, w, b, out_dtype):
-    if torch.is_grad_enabled():
+    if torch.is_grad_enabled() or _forward_mode():
         return _AffineFp8.apply(x, w, b, out_dtype)
     if x.shape[1] != w.shape[1]:
         raise ValueError('dense: inputs %s against weights %s' % (tuple(x.shape), tuple(w.shape)))
@@ -362,7 +369,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     -> x's shape and type; differentiable in all three (csrc/layernorm.hip: one pass each way)."""
     _need_gpu(x)
     rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])           # (no views in autograd's graph where none are needed)
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
+    if _forward_mode() or (torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
+                                                        (bias is not None and bias.requires_grad))):
         y = _LayerNorm.apply(rows, weight, bias, eps)
     else:
         y = ops._layer_norm(_row_form(rows), weight, bias, eps, False)[0]

@@ -32,3 +32,24 @@ def test_fp8_layers_refuse_another_width(stubbed, grad):
                 lin(torch.randn(3, width))
             with pytest.raises(ValueError):
                 stubbed.affine(torch.randn(2, 3, width), lin.weight)
+
+
+@pytest.mark.parametrize('grad', [True, False])
+@pytest.mark.parametrize('which', ['input', 'weight', 'bias'])
+def test_forward_mode_tangents_are_not_dropped(stubbed, monkeypatch, grad, which):
+    """a dual tensor, whatever it is an argument of and whether or not a backward is recorded: no layer answers without its derivative"""
+    import torch.autograd.forward_ad as fwd
+    from sgg_amd import ops
+    monkeypatch.setattr(ops, '_layer_norm', lambda x, w, b, eps, stats: (x * 1.0, torch.zeros(2, x.shape[0])))
+    args = {'input': torch.randn(3, 7), 'weight': torch.randn(7, 7), 'bias': torch.randn(7)}
+    vec = {'input': args['input'], 'weight': torch.randn(7), 'bias': args['bias']}
+    calls = (lambda a, v: stubbed.layer_norm(v['input'], v['weight'], v['bias']), lambda a, v: stubbed.affine_fp8(a['input'], a['weight'], a['bias']),
+             lambda a, v: stubbed.affine(a['input'], a['weight'], a['bias']))
+    with torch.set_grad_enabled(grad):
+        for call in calls:
+            call(args, vec)
+            with fwd.dual_level():
+                call(args, vec)                                              # nothing carries a tangent: as outside
+                dual = [{k: fwd.make_dual(v, torch.ones_like(v)) if k == which else v for k, v in d.items()} for d in (args, vec)]
+                with pytest.raises(Exception, match='jvp'):
+                    call(*dual)
