@@ -47,9 +47,9 @@ def compute_mode():
     return _COMPUTE[0]
 
 
-def product(x, w, bias=None):
-    """x [M,Kp] f32 . w [N,Kp]^T (+ bias) -> [M,N] f32 in the file's arithmetic (Kp a multiple of 32, zero-padded)"""
-    mode = _COMPUTE[0]
+def product(x, w, bias=None, mode=None):
+    """x [M,Kp] f32 . w [N,Kp]^T (+ bias) -> [M,N] f32 in the file's arithmetic (Kp a multiple of 32, zero-padded), or in `mode`'s"""
+    mode = mode or _COMPUTE[0]
     if mode == 'fp8':
         return ops.gemm_fp8(ops.quantize_fp8(x), ops.quantize_fp8(w), bias)
     if mode == 'f16':
@@ -98,14 +98,16 @@ class _Affine(torch.autograd.Function):
             raise ValueError('dense: %d input columns against %d weight columns' % (x.shape[1], w.shape[1]))
         ctx.save_for_backward(xp, wp)
         ctx.dims = (x.shape[1], w.shape[0], w.shape[1], b is not None)
+        ctx.mode = _COMPUTE[0]
         if xp.shape[0] == 0:
             return xp.new_zeros((0, w.shape[0]))
-        return product(xp, wp, b.detach().float().contiguous() if b is not None else None)
+        return product(xp, wp, b.detach().float().contiguous() if b is not None else None, ctx.mode)
 
     @staticmethod
     def backward(ctx, dy):
         xp, wp = ctx.saved_tensors
         Kx, N, K, has_b = ctx.dims
+        mode = ctx.mode if _COMPUTE[0] == 'fp8' else _COMPUTE[0]        # (8 bits only for what was multiplied in 8 bits)
         M = xp.shape[0]
         dx = dw = db = None
         if M == 0:
@@ -114,10 +116,10 @@ class _Affine(torch.autograd.Function):
         dy = dy.contiguous().float()
         if ctx.needs_input_grad[0]:
             wt = ops.transpose(wp, pad_to=32)                           # [Kp, N32]
-            dx = product(_cols32(dy), wt)[:, :Kx]
+            dx = product(_cols32(dy), wt, mode=mode)[:, :Kx]
         if ctx.needs_input_grad[1]:
             # dW = dy^T x: both operands transposed once (zero-padded reduction rows), then the same GEMM
-            dw = product(ops.transpose(dy), ops.transpose(xp))[:, :K]
+            dw = product(ops.transpose(dy), ops.transpose(xp), mode=mode)[:, :K]
         if has_b and ctx.needs_input_grad[2]:
             db = ops.colsum(dy)
         return dx, dw, db

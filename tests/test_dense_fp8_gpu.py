@@ -1,0 +1,62 @@
+"""The 'fp8' arithmetic of the dense layers on the GPU: the row product itself, widths that do not fit, a mode switched between forward and backward."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda:0'
+U = 2.0 ** -24
+
+
+@pytest.fixture(autouse=True)
+def mode():
+    from sgg_amd import dense
+    prev = dense.compute_mode()
+    yield
+    dense.set_compute(prev)
+
+
+@pytest.mark.parametrize('M,K,N', [(1, 32, 5), (40, 64, 70), (300, 1056, 129)])
+def test_product_is_the_product_of_the_8_bit_forms(M, K, N):
+    """fp32 sums of whole products: (K + 32) 2^-24 of the sum of magnitudes, the bias one rounding more"""
+    from sgg_amd import dense, ops
+    torch.manual_seed(M)
+    x, w, b = torch.randn(M, K, device=DEV), torch.randn(N, K, device=DEV), torch.randn(N, device=DEV)
+    dense.set_compute('fp8')
+    y = dense.product(x, w, b)
+    a, c = ops.quantize_fp8(x).dequantize(), ops.quantize_fp8(w).dequantize()
+    tol = (K + 33) * U * (torch.mm(a.abs(), c.abs().t().contiguous()) + b.double().abs())
+    assert y.dtype == torch.float32 and bool(((y.double() - torch.mm(a, c.t().contiguous()) - b.double()).abs() <= tol).all())
+    dense.set_compute('f32')
+    assert torch.equal(dense.product(x, w, b, mode='fp8'), y)
+
+
+def test_a_mode_switched_between_forward_and_backward():
+    from sgg_amd import dense
+    torch.manual_seed(1)
+    x = torch.randn(70, 96, device=DEV, requires_grad=True)
+    lin = dense.Linear(96, 40).to(DEV)
+    dy = torch.randn(70, 40, device=DEV)
+    leaves = (x, lin.weight, lin.bias)
+
+    def grads(forward, backward):
+        dense.set_compute(forward)
+        y = lin(x)
+        dense.set_compute(backward)
+        return torch.autograd.grad(y, leaves, dy)
+    for other in ('f32', 'x3', 'f16'):
+        for a, b in zip(grads(other, 'fp8'), grads(other, other)):
+            assert torch.equal(a, b)
+        for a, b in zip(grads('fp8', other), grads('fp8', 'fp8')):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('grad', [True, False])
+def test_widths_that_do_not_fit_are_refused(grad):
+    from sgg_amd import dense
+    dense.set_compute('fp8')
+    lin = dense.Linear(100, 5).to(DEV)
+    with torch.set_grad_enabled(grad):
+        for width in (64, 99, 101, 130):
+            with pytest.raises(ValueError):
+                lin(torch.randn(3, width, device=DEV))
+        assert lin(torch.randn(2, 3, 100, device=DEV)).shape == (2, 3, 5)

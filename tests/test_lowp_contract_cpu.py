@@ -53,3 +53,28 @@ def test_forward_mode_tangents_are_not_dropped(stubbed, monkeypatch, grad, which
                 dual = [{k: fwd.make_dual(v, torch.ones_like(v)) if k == which else v for k, v in d.items()} for d in (args, vec)]
                 with pytest.raises(Exception, match='jvp'):
                     call(*dual)
+
+
+@pytest.mark.parametrize('forward,backward,want', [('f32', 'fp8', 'f32'), ('x3', 'fp8', 'x3'), ('f16', 'fp8', 'f16'), ('f32', 'f16', 'f16'), ('f32', 'f32', 'f32')])
+def test_a_backward_is_not_done_in_8_bits_unless_its_forward_was(monkeypatch, forward, backward, want):
+    """set_compute between a forward and its backward"""
+    from sgg_amd import dense, ops
+    seen = []
+
+    def product(x, w, bias=None, mode=None):
+        seen.append(mode or dense.compute_mode())
+        return x @ w.t()
+    monkeypatch.setattr(dense, '_need_gpu', lambda x: None)
+    monkeypatch.setattr(dense, 'product', product)
+    monkeypatch.setattr(ops, 'transpose', lambda t, pad_to=1: torch.nn.functional.pad(t.t(), (0, -t.shape[0] % 32)).contiguous())
+    x, w = torch.randn(5, 32, requires_grad=True), torch.randn(7, 32, requires_grad=True)
+    prev = dense.set_compute(forward)
+    try:
+        y = dense.affine(x, w)
+        dense.set_compute(backward)
+        dy = torch.randn(5, 7)
+        dx, dw = torch.autograd.grad(y, (x, w), dy)
+    finally:
+        dense.set_compute(prev)
+    assert seen == [forward, want, want]
+    assert torch.allclose(dx, dy @ w) and torch.allclose(dw, dy.t() @ x, atol=1e-5)
