@@ -360,10 +360,12 @@ class _LayerNorm(torch.autograd.Function):
     def backward(ctx, dy):
         x, stats, w = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dy = dy if dy.is_contiguous() else _row_form(dy)             # (autograd has seen to shape, type and device; x and w were checked on the way in)
+        dy = dy if dy.is_contiguous() else _row_form(dy)             # (autograd has seen to dy's shape, type and device)
         C, mean = x.shape[1], stats.data_ptr()
-        return ops._layer_norm_bwd(dy, max(dy.stride(0), C), x, max(x.stride(0), C), mean, mean + 4 * x.shape[0], None if w is None else w.data_ptr(),
-                                   need[0], need[1], need[2]) + (None,)
+        # the weight is the caller's own: module.cpu() or .half() since the forward leaves other memory behind its name, which no version counter tells
+        wp = ops._vector(w, C, 'layer_norm weight in the backward')
+        ops._here(x, 'layer_norm backward')
+        return ops._layer_norm_bwd(dy, max(dy.stride(0), C), x, max(x.stride(0), C), mean, mean + 4 * x.shape[0], wp, need[0], need[1], need[2]) + (None,)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):

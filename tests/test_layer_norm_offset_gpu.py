@@ -122,3 +122,22 @@ def test_differences_whose_squares_pass_fp32(C, dtype):
     held(x, w, b, dy)
     y = ops.layer_norm(x, w, b)[0]
     assert torch.equal(ops.layer_norm(x[5:40], w, b)[0], y[5:40])
+
+
+def test_a_weight_changed_between_forward_and_backward_is_refused():
+    """another type, another device or fewer columns behind the saved parameter: an error, no launch; an in-place change is autograd's own"""
+    from sgg_amd import dense
+    x = torch.randn(30, 64, device=DEV, requires_grad=True)
+    for change, error in ((lambda w: w.half(), TypeError), (lambda w: w.cpu(), RuntimeError), (lambda w: w[:32].clone(), ValueError),
+                          (lambda w: w.expand(2, 64), ValueError)):
+        m = dense.LayerNormRows(64).to(DEV)
+        y = m(x)
+        m.weight.data = change(m.weight.data)
+        with pytest.raises(error):
+            y.sum().backward()
+    m = dense.LayerNormRows(64).to(DEV)
+    y = m(x)
+    with torch.no_grad():
+        m.weight.mul_(2)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.sum().backward()

@@ -78,3 +78,18 @@ def test_a_backward_is_not_done_in_8_bits_unless_its_forward_was(monkeypatch, fo
         dense.set_compute(prev)
     assert seen == [forward, want, want]
     assert torch.allclose(dx, dy @ w) and torch.allclose(dw, dy.t() @ x, atol=1e-5)
+
+
+def test_a_weight_that_is_elsewhere_by_the_time_of_the_backward(monkeypatch):
+    """module.cpu() between forward and backward gives the saved parameter other memory under the same name and version: its address must not reach
+    a kernel (here every tensor is on the CPU, as that one would be)"""
+    from sgg_amd import dense, ops
+    monkeypatch.setattr(dense, '_need_gpu', lambda x: None)
+    monkeypatch.setattr(ops, '_layer_norm', lambda x, w, b, eps, stats: (x * 1.0, torch.zeros(2, x.shape[0])))
+    launched = []
+    monkeypatch.setattr(ops, '_layer_norm_bwd', lambda *a: (launched.append(a), (None, None, None))[1])
+    x, m = torch.randn(3, 7, requires_grad=True), dense.LayerNormRows(7)
+    y = m(x)
+    with pytest.raises(RuntimeError, match='not on the GPU'):
+        y.sum().backward()
+    assert not launched
