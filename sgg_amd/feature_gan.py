@@ -392,6 +392,19 @@ def allreduce_grads_(params, scale=1.0):
                 p.grad.mul_(scale)
 
 
+def _clip_gradients(parameters, max_norm):
+    """the gradients' global norm clipped on trainer.clip_grad_norm_'s kernels, or by torch's function where those do not take them: fp64, rows with
+    gaps, memory that two of them share, other devices.  (What the kernels refuse they refuse before any launch.)"""
+    from .trainer import clip_grad_norm_
+    params = [p for p in parameters if p.grad is not None]
+    if all(p.grad.is_cuda and p.grad.get_device() == torch.cuda.current_device() for p in params):
+        try:
+            return clip_grad_norm_(params, max_norm)
+        except (TypeError, ValueError):
+            pass
+    return torch.nn.utils.clip_grad_norm_(params, max_norm)
+
+
 def gan_train_step(sgg_model, gan, res, gt_boxes, gt_objects, gt_rels, optimizer, G_optimizer, D_optimizer, *, ganw=1.0,
                    attachG=False, ganlosses=('D', 'G', 'rec'), loss_type='baseline', loss_weights=(1, 1, 1), clip=5.0,
                    gt_objects_fake=None, trainer=None):
@@ -414,7 +427,7 @@ def gan_train_step(sgg_model, gan, res, gt_boxes, gt_objects, gt_rels, optimizer
     BatchNorm1d of the graph convolutions when BN=True) use batch statistics: convert them with
     `sgg_amd.dense.sync_batchnorm_(gan)` (the channels-last counterpart of torch.nn.SyncBatchNorm.convert_sync_batchnorm) for
     statistics over every rank's images (what the test does), or keep replica-local statistics."""
-    from .trainer import Trainer, clip_grad_norm_
+    from .trainer import Trainer
     import torch.distributed as dist
     world = _dp_world()
     gan.train()
@@ -481,7 +494,7 @@ def gan_train_step(sgg_model, gan, res, gt_boxes, gt_objects, gt_rels, optimizer
                 else:
                     allreduce_grads_([p for p in sgg_model.parameters() if p.requires_grad])
                     if clip:
-                        clip_grad_norm_(sgg_model.parameters(), clip)
+                        _clip_gradients(sgg_model.parameters(), clip)
                     optimizer.step()
             allreduce_grads_(G_params, 1.0 / scale)
             # a scaled f16 backward that overflowed: the SGG update above was skipped by its norm check; the generator's optimiser has no

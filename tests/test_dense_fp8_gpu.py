@@ -60,3 +60,24 @@ def test_widths_that_do_not_fit_are_refused(grad):
             with pytest.raises(ValueError):
                 lin(torch.randn(3, width, device=DEV))
         assert lin(torch.randn(2, 3, 100, device=DEV)).shape == (2, 3, 5)
+
+
+def test_gan_iteration_clips_any_gradients():
+    """ordinary ones on the kernels; fp64, rows with gaps and one gradient of two parameters as torch's function does"""
+    from sgg_amd.feature_gan import _clip_gradients
+
+    def params(kind):
+        torch.manual_seed(0)
+        ps = [torch.nn.Parameter(torch.zeros(40, 40, device=DEV, dtype=torch.float64 if kind == 'double' and i else torch.float32)) for i in range(3)]
+        for p in ps:
+            p.grad = torch.randn(40, 80, device=DEV)[:, ::2].to(p.dtype) if kind == 'gaps' else torch.randn(40, 40, device=DEV).to(p.dtype)
+        if kind == 'shared':
+            ps[1].grad = ps[0].grad
+        return ps
+    for kind in ('plain', 'double', 'gaps', 'shared'):
+        mine, ref = params(kind), params(kind)
+        assert kind != 'gaps' or not mine[0].grad.is_contiguous()
+        n, r = _clip_gradients(mine, 0.5), torch.nn.utils.clip_grad_norm_(ref, 0.5)
+        assert abs(float(n) - float(r)) <= 2404 * U * float(r)              # (torch: 4800 fp32 squares, a rounding each at most, their root half of that)
+        for a, b in zip(mine, ref):
+            assert float((a.grad - b.grad).abs().max()) <= 2408 * U * float(b.grad.abs().max())

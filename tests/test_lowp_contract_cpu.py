@@ -93,3 +93,19 @@ def test_a_weight_that_is_elsewhere_by_the_time_of_the_backward(monkeypatch):
     with pytest.raises(RuntimeError, match='not on the GPU'):
         y.sum().backward()
     assert not launched
+
+
+def test_gan_iteration_clips_what_the_kernels_do_not_take():
+    """fp64, gaps, a gradient that two parameters share, memory on the host: as torch's function clips them"""
+    from sgg_amd.feature_gan import _clip_gradients
+
+    def params():
+        torch.manual_seed(0)
+        ps = [torch.nn.Parameter(torch.zeros(4, 4, dtype=t)) for t in (torch.float32, torch.float64, torch.float32, torch.float32, torch.float32)]
+        grads = [torch.randn(4, 4), torch.randn(4, 4).double(), torch.randn(4, 8)[:, ::2], torch.randn(4, 4)]
+        for p, g in zip(ps, grads):
+            p.grad = g
+        return ps
+    mine, ref = params(), params()
+    assert torch.equal(_clip_gradients(iter(mine), 0.5), torch.nn.utils.clip_grad_norm_(ref, 0.5))
+    assert all(torch.equal(a.grad, b.grad) for a, b in zip(mine[:4], ref[:4])) and mine[4].grad is None
