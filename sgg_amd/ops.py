@@ -1297,19 +1297,21 @@ class Fp8Rows(object):
 
     def codes(self):
         """-> float8_e4m3fn [M, K rounded up to 128], the rows as rows"""
-        return self.data[:, :self.shape[0]].transpose(0, 1).reshape(self.shape[0], -1)
+        M, blocks = self.shape[0], (self.shape[1] + FP8_BLOCK - 1) // FP8_BLOCK
+        return self.data[:, :M].transpose(0, 1).reshape(M, blocks * FP8_BLOCK)
 
     def exponents(self):
         """-> int32 [M, blocks]: block b of row m stands for its e4m3 values times 2^exponents[m, b]"""
         M, blocks = self.shape[0], (self.shape[1] + FP8_BLOCK - 1) // FP8_BLOCK
-        e = self.scale.view(blocks, -1, 32, 4).permute(1, 3, 2, 0).reshape(-1, blocks)        # (block, group, r % 32, r / 32) -> rows
+        groups = (M + 127) // 128
+        e = self.scale.view(blocks, groups, 32, 4).permute(1, 3, 2, 0).reshape(groups * 128, blocks)        # (block, group, r % 32, r / 32) -> rows
         return e[:M].int() - 127
 
     def dequantize(self):
         """-> f64 [M, K], the values the operand stands for, each of them exact (fp32's largest rounds to 2^128, which fp32 has not)"""
         M, K = self.shape
         e = ((self.exponents().long() + 1023) << 52).view(torch.float64)                      # 2^e itself
-        return (self.codes().float().double().view(M, -1, FP8_BLOCK) * e[:, :, None]).reshape(M, -1)[:, :K]
+        return (self.codes().float().double().view(M, e.shape[1], FP8_BLOCK) * e[:, :, None]).view(M, e.shape[1] * FP8_BLOCK)[:, :K]
 
 
 def _fp8_dims(M, K):

@@ -109,3 +109,14 @@ def test_gan_iteration_clips_what_the_kernels_do_not_take():
     mine, ref = params(), params()
     assert torch.equal(_clip_gradients(iter(mine), 0.5), torch.nn.utils.clip_grad_norm_(ref, 0.5))
     assert all(torch.equal(a.grad, b.grad) for a, b in zip(mine[:4], ref[:4])) and mine[4].grad is None
+
+
+@pytest.mark.parametrize('M,K', [(0, 0), (0, 200), (3, 0), (1, 1), (129, 130)])
+def test_operand_forms_of_no_rows_or_columns_can_be_read(M, K):
+    from sgg_amd import ops
+    slabs, R, scales = ops._fp8_dims(M, K)
+    blocks = (K + 127) // 128
+    for q in (ops.Fp8Rows._of(torch.full((slabs * R * 64 + scales,), 127, dtype=torch.uint8), (M, K)),
+              ops.Fp8Rows(torch.zeros(slabs, R, 64, dtype=torch.uint8).view(torch.float8_e4m3fn), torch.full((scales,), 127, dtype=torch.uint8), (M, K))):
+        assert q.codes().shape == (M, blocks * 128) and q.exponents().shape == (M, blocks) and q.dequantize().shape == (M, K)
+        assert not q.exponents().any()
