@@ -393,16 +393,15 @@ def allreduce_grads_(params, scale=1.0):
 
 
 def _clip_gradients(parameters, max_norm):
-    """the gradients' global norm clipped on trainer.clip_grad_norm_'s kernels, or by torch's function where those do not take them: fp64, rows with
-    gaps, memory that two of them share, other devices.  (What the kernels refuse they refuse before any launch.)"""
+    """the gradients' global norm clipped on trainer.clip_grad_norm_'s kernels, or by torch's function where one of them is not theirs to take: fp64, a
+    layout with gaps, another device.  (Gradients that share memory are refused: torch's scales them once or twice, as its threads happen to run.)"""
+    from . import ops
     from .trainer import clip_grad_norm_
     params = [p for p in parameters if p.grad is not None]
-    if all(p.grad.is_cuda and p.grad.get_device() == torch.cuda.current_device() for p in params):
-        try:
-            return clip_grad_norm_(params, max_norm)
-        except (TypeError, ValueError):
-            pass
-    return torch.nn.utils.clip_grad_norm_(params, max_norm)
+    here = torch.cuda.current_device() if any(p.grad.is_cuda for p in params) else None
+    theirs = all(p.grad.is_cuda and p.grad.get_device() == here and p.grad.dtype in (torch.float32, torch.bfloat16, torch.float16) and
+                 ops._dense_layout(p.grad) for p in params)
+    return (clip_grad_norm_ if theirs else torch.nn.utils.clip_grad_norm_)(params, max_norm)
 
 
 def gan_train_step(sgg_model, gan, res, gt_boxes, gt_objects, gt_rels, optimizer, G_optimizer, D_optimizer, *, ganw=1.0,

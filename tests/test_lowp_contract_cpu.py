@@ -96,7 +96,7 @@ def test_a_weight_that_is_elsewhere_by_the_time_of_the_backward(monkeypatch):
 
 
 def test_gan_iteration_clips_what_the_kernels_do_not_take():
-    """fp64, gaps, a gradient that two parameters share, memory on the host: as torch's function clips them"""
+    """fp64, gaps, memory on the host: as torch's function clips them"""
     from sgg_amd.feature_gan import _clip_gradients
 
     def params():
