@@ -15,6 +15,7 @@ normalisation), so the reference's checkpoints load by name.
 The kernels run on the GPU only: a CPU tensor raises (there is no fallback path).
 """
 import functools
+import math
 
 import torch
 import torch.nn as nn
@@ -132,6 +133,11 @@ def _row_form(x):
     return x if (K <= 1 or x.stride(1) == 1) and (M <= 1 or x.stride(0) >= K) else x.contiguous()
 
 
+def _rows(x):
+    """x [..., C] as a row matrix [rows, C] (a matrix as it is: no view in autograd's graph; also where there are no columns, which reshape(-1, 0) refuses)"""
+    return x if x.dim() == 2 else x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
+
+
 def _gemm_rows(x, w, b, out_dtype):
     b = None if b is None else b.detach().float().contiguous()
     return ops._gemm_fp8(x, w, ops._vector(b, w.shape[0], 'dense bias'), out_dtype=out_dtype)
@@ -185,7 +191,7 @@ class _AffineFp8(torch.autograd.Function):
             if need_dx:
                 dq = ops.quantize_fp8(dy)
             if need_db:
-                db = ops.colsum(dy.contiguous()) if dy.shape[0] else dy.new_zeros(dy.shape[1], dtype=torch.float32)
+                db = ops.colsum(dy.contiguous()) if dy.numel() else dy.new_zeros(dy.shape[1], dtype=torch.float32)
         if need_dx:
             dx = ops._gemm_fp8(dq, wt, out_dtype=ctx.types[0])
         if need_dw:
@@ -200,9 +206,8 @@ def affine_fp8(x, weight, bias=None, out_dtype=None):
     results and up to 32 rows), out_dtype (default x's type); differentiable in all three, the gradients' products in 8 bits too: dx in x's type,
     the weight's always through f32.  What set_compute('fp8') makes of affine / conv2d, with f32 results."""
     _need_gpu(x)
-    if x.dim() == 2:                                 # (no views in autograd's graph: ~10 us of the host's each way)
-        return _affine_fp8_rows(x, weight, bias, out_dtype or x.dtype)
-    return _affine_fp8_rows(x.reshape(-1, x.shape[-1]), weight, bias, out_dtype or x.dtype).view(*x.shape[:-1], weight.shape[0])
+    y = _affine_fp8_rows(_rows(x), weight, bias, out_dtype or x.dtype)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], weight.shape[0])          # (no views in autograd's graph: ~10 us of the host's each way)
 
 
 def _affine_fp8_rows(x, w, b, out_dtype):
@@ -222,9 +227,7 @@ def _affine_rows(x, w, b):
 
 def affine(x, weight, bias=None):
     """x [..., K] -> [..., N] = x . weight^T + bias (weight [N,K]) on sgg_gemm (sgg_gemm_fp8 in the 'fp8' arithmetic); differentiable in all three."""
-    lead = x.shape[:-1]
-    y = _affine_rows(x.reshape(-1, x.shape[-1]), weight, bias)
-    return y.view(*lead, weight.shape[0])
+    return _affine_rows(_rows(x), weight, bias).view(*x.shape[:-1], weight.shape[0])
 
 
 class _Patches(torch.autograd.Function):
@@ -372,7 +375,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Layer normalisation over the last axis of x [..., C] (f32 / bf16 / f16; statistics and sums in fp32) with weight, bias f32[C] or None
     -> x's shape and type; differentiable in all three (csrc/layernorm.hip: one pass each way)."""
     _need_gpu(x)
-    rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])           # (no views in autograd's graph where none are needed)
+    rows = _rows(x)
     if _forward_mode() or (torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
                                                         (bias is not None and bias.requires_grad))):
         y = _LayerNorm.apply(rows, weight, bias, eps)

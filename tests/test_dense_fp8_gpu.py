@@ -86,3 +86,31 @@ def test_gan_iteration_clips_any_gradients():
     with pytest.raises(ValueError):
         _clip_gradients(ps, 0.5)
     assert all(torch.equal(p.grad, g) for p, g in zip(ps, before))
+
+
+@pytest.mark.parametrize('shape,N', [((2, 3, 0), 5), ((0,), 5), ((3, 0), 5), ((2, 0, 7), 5), ((4, 7), 0), ((33, 7), 0), ((0, 0), 0)])
+def test_no_rows_columns_or_outputs(shape, N):
+    """forward and every gradient of a product with a length of zero; the operand forms' own readings"""
+    from sgg_amd import dense, ops
+    K = shape[-1]
+    x = torch.randn(shape, device=DEV, requires_grad=True)
+    w, b = torch.randn(N, K, device=DEV, requires_grad=True), torch.randn(N, device=DEV, requires_grad=True)
+    dense.set_compute('fp8')
+    for call in (dense.affine_fp8, dense.affine):
+        y = call(x, w, b)
+        dy = torch.randn_like(y)
+        dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+        assert y.shape == shape[:-1] + (N,) and dx.shape == shape and dw.shape == (N, K) and db.shape == (N,)
+        want = b.detach().expand_as(y) if not K else y.detach()
+        assert torch.equal(y.detach(), want) and not dw.any() and (N or not dx.any())
+        assert float((db - dy.reshape(dy.numel() // N if N else 0, N).sum(0)).abs().sum()) <= 1e-5
+        assert torch.autograd.grad(call(x.detach(), w.detach(), b), b, dy)[0].shape == (N,)
+    for q in ops.quantize_fp8(torch.zeros(shape[-2] if len(shape) > 1 else 1, K, device=DEV), 'both'):
+        assert q.codes().shape[0] == q.shape[0] and q.exponents().shape[0] == q.shape[0] and q.dequantize().shape == q.shape
+
+
+def test_layer_norm_of_no_columns_is_refused():
+    from sgg_amd import dense
+    for shape in ((3, 0), (2, 3, 0), (0,)):
+        with pytest.raises(ValueError):
+            dense.layer_norm(torch.zeros(shape, device=DEV))

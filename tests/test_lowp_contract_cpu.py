@@ -120,3 +120,10 @@ def test_operand_forms_of_no_rows_or_columns_can_be_read(M, K):
               ops.Fp8Rows(torch.zeros(slabs, R, 64, dtype=torch.uint8).view(torch.float8_e4m3fn), torch.full((scales,), 127, dtype=torch.uint8), (M, K))):
         assert q.codes().shape == (M, blocks * 128) and q.exponents().shape == (M, blocks) and q.dequantize().shape == (M, K)
         assert not q.exponents().any()
+
+
+def test_8_bit_layers_of_no_columns_give_the_bias(stubbed):
+    for shape in ((0,), (3, 0), (2, 3, 0), (2, 0, 4, 0)):
+        for call in (stubbed.affine_fp8, stubbed.affine):
+            assert call(torch.zeros(shape), torch.zeros(5, 0)).shape == shape[:-1] + (5,)
+    assert stubbed.affine_fp8(torch.zeros(2, 0, 7), torch.zeros(5, 7)).shape == (2, 0, 5)
