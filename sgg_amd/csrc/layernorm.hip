@@ -413,7 +413,8 @@ __global__ __launch_bounds__(256) void ln_dw_sum_kernel(const float* __restrict_
     else if ((C) <= 8192) { using S = LnShape<64, 8, 2>; __VA_ARGS__; }        \
     else { using S = LnShape<64, 16, 2>; __VA_ARGS__; }
 
-// workgroups: enough rows for all, at most `waves` waves per CU
+// workgroups: enough rows for all, at most `waves` waves per CU.  Forward 16 (65536 x 4096 bf16 197 us; 8 waves: 245, 32: 205; f32 496, 492, 417),
+// backward 8, whose workgroups each leave a row of partial column sums to join (308 us; 4 waves: 482, 16: 330; 7936 x 512 f16 11.7, 12.2, 13.9)
 template <typename S>
 int ln_blocks(int64_t M, int waves) {
     const int64_t most = 256 * (int64_t)(waves / S::WAVES > 0 ? waves / S::WAVES : 1);
