@@ -114,3 +114,45 @@ def test_layer_norm_of_no_columns_is_refused():
     for shape in ((3, 0), (2, 3, 0), (0,)):
         with pytest.raises(ValueError):
             dense.layer_norm(torch.zeros(shape, device=DEV))
+
+
+def test_gan_iteration_in_8_bits_with_clipped_gradients():
+    """a whole iteration: the generator's and the discriminators' layers in the fp8 arithmetic, the relation model's gradients clipped before an
+    optimiser that is not FusedSGD; every part learns, and the same iteration gives the same weights (but for the two discriminators' first layers: the
+    gradient of their lookup of class columns is an indexed sum of torch's, in the order its threads run -- in every arithmetic)"""
+    import sgg_amd
+    from sgg_amd import dense
+    from sgg_amd.feature_gan import GAN, gan_train_step
+    from sgg_amd.synthetic import SyntheticData, init_weights, synthetic_batch
+
+    def iteration():
+        torch.manual_seed(3)
+        data = SyntheticData()
+        model = init_weights(sgg_amd.RelModelStanford(data, mode='sgcls')).to(DEV)
+        model.set_compute_dtype(torch.float32)
+        for n, p in model.named_parameters():
+            if n.startswith('detector.'):
+                p.requires_grad = False
+        gan = GAN(data.ind_to_classes, data.ind_to_predicates, n_ch=model.edge_dim, pool_sz=model.pool_sz, fmap_sz=model.fmap_sz, n_layers_G=2,
+                  device=DEV).to(DEV)
+        batch = tuple(t.to(DEV) if isinstance(t, torch.Tensor) else t for t in synthetic_batch(B=2, n_boxes=5, n_fg=4, seed=8))
+        model.train()
+        res = model([batch])
+        opt = torch.optim.SGD([p for p in model.parameters() if p.requires_grad], lr=1e-3)
+        G_opt = torch.optim.SGD([p for n, p in gan.named_parameters() if n.startswith('G_')], lr=1e-2)
+        D_opt = torch.optim.SGD([p for n, p in gan.named_parameters() if n.startswith('D_')], lr=1e-2)
+        named = dict([('sgg.' + n, p) for n, p in model.named_parameters() if p.requires_grad] + list(gan.named_parameters()))
+        before = {n: p.detach().clone() for n, p in named.items()}
+        losses = gan_train_step(model, gan, res, batch[3].clone(), batch[4].clone(), batch[5].clone(), opt, G_opt, D_opt, clip=0.1)
+        assert all(torch.isfinite(v) for v in losses.values())
+        for n, p in named.items():
+            assert bool(torch.isfinite(p).all()) and (p.grad is None or bool(torch.isfinite(p.grad).all())), n
+        step = sum((p.detach().double() - before[n].double()).square().sum() for n, p in named.items() if n.startswith('sgg.')) ** 0.5
+        assert 0 < float(step) <= 1e-3 * 0.1 * 1.01                       # lr times the clipped norm (and the weights' own rounding)
+        for must in ('G_obj_embed.weight', 'G_gcn.gconvs.0.net1.0.weight', 'G_node.0.weight', 'G_proj.weight', 'G_refine.output_conv.0.weight',
+                     'D_nodes.0.weight_orig', 'D_edges.6.weight_orig', 'D_global.15.weight_orig', 'sgg.rel_fc.weight', 'sgg.roi_fmap.1.0.weight'):
+            assert not torch.equal(before[must], named[must].detach()), must
+        return {n: p.detach().clone() for n, p in named.items()}
+    dense.set_compute('fp8')
+    a, b = iteration(), iteration()
+    assert [n for n in a if not torch.equal(a[n], b[n]) and n not in ('D_nodes.0.weight_orig', 'D_edges.0.weight_orig')] == []
