@@ -366,8 +366,10 @@ class _LayerNorm(torch.autograd.Function):
         dy = dy if dy.is_contiguous() else _row_form(dy)             # (autograd has seen to dy's shape, type and device)
         C, mean = x.shape[1], stats.data_ptr()
         # the weight is the caller's own: module.cpu() or .half() since the forward leaves other memory behind its name, which no version counter tells
-        wp = ops._vector(w, C, 'layer_norm weight in the backward')
-        ops._here(x, 'layer_norm backward')
+        if not x.is_cuda or (w is not None and (w.dtype is not torch.float32 or w.get_device() != x.get_device() or w.shape != x.shape[1:] or not w.is_contiguous())):
+            ops._here(x, 'layer_norm backward')
+            ops._vector(w, C, 'layer_norm weight in the backward')                 # (says which)
+        wp = None if w is None else w.data_ptr()
         return ops._layer_norm_bwd(dy, max(dy.stride(0), C), x, max(x.stride(0), C), mean, mean + 4 * x.shape[0], wp, need[0], need[1], need[2]) + (None,)
 
 
