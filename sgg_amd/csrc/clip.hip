@@ -4,7 +4,7 @@
 // there to its type (the chip has no way from 64 bits to 16): at most 2^-24 of it beside its own half step.
 // No atomics: one partial per workgroup, added in a fixed order -- the same gradients give the same bits every time.
 // Memory-bound, two readings and one writing (the factor is known only after the first).  Measured: 40 tensors of 248 M fp32 elements: norm 162 us (6.1 TB/s),
-// scaling 404 us (4.9 TB/s, a copy's rate); 32 tensors of 17 M elements fp16 -> fp32: 12 + 31 us; 8 tensors of 17 K elements: 4 + 5 us.
+// scaling 382 .. 407 us (4.9 .. 5.2 TB/s, a copy's rate); 32 tensors of 17 M elements fp16 -> fp32: 12 + 30 us; 8 tensors of 17 K elements: 4 + 5 us.
 #include <algorithm>
 #include <memory>
 #include <new>
